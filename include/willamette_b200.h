@@ -59,6 +59,7 @@ typedef enum wl_status {
 #define WL_GGML_Q8_0 8u
 #define WL_GGML_Q4_K 12u
 #define WL_GGML_Q6_K 14u
+#define WL_GGML_BF16 30u
 #define WL_GGML_I2_S 36u
 
 /* Layout constants (src/gguf/tensor.rs:86-105, :141-175). */
@@ -100,7 +101,8 @@ int wl_init(int device);
 /* Free every cached device copy of host weights. */
 int wl_release_weights(void);
 /* Device-side error word (bit 0: a bounded wait timed out; bit 1: a
- * tensor-parallel peer never arrived).  Synchronises the device, then reads
+ * tensor-parallel peer never arrived; bit 2: an attention operator read a
+ * page id, position, length or sequence extent outside its range).  Synchronises the device, then reads
  * and clears it.  Includes the status word of wl_dev_i2s_matvec_f32_noalloc
  * on the calling thread's current device; when only that entry point has run
  * in the process, this call allocates nothing either. */
@@ -330,6 +332,116 @@ int wl_dev_i2s_matvec_f32(const uint8_t *packed, float w_scale, uint32_t in_dim,
 #define WL_NOALLOC_MAX_IN_DIM 16384u
 int wl_dev_i2s_matvec_f32_noalloc(const uint8_t *packed, float w_scale, uint32_t in_dim,
                                   uint32_t out_dim, const float *x, float *y, void *stream);
+
+/* ------------------------------- attention over a paged int8 KV cache, prompts
+ * Operators a serving loop composes into its own forward over buffers of its
+ * own (the engines below hold their cache themselves): rotate and append a
+ * step's or a prompt's keys and values, attend over the cache with one token
+ * per sequence, attend within packed prompts.  No counterpart in the
+ * reference (its KV cache is one contiguous block per sequence with a scale
+ * per token, src/model/kv_cache.rs:245-259).  Asynchronous on `stream`,
+ * capturable in CUDA graphs (call wl_init or any wl_dev_* call first); the
+ * current device must be the library's.  head_dim is 64 or 128
+ * (WL_ERR_NOT_IMPLEMENTED otherwise), query heads a multiple of the KV heads:
+ * query head h reads KV head h / (n_q_heads / n_kv_heads).  Row buffers
+ * (q, k, v, out) hold token t's heads side by side at t * stride elements;
+ * they are 16-byte aligned, strides multiples of 16 bytes, so that slices of
+ * one fused projection work.  Page ids, positions, lengths and seq_start are
+ * read on the device: a value outside its range is left out and sets bit 2
+ * of wl_device_status, never followed. */
+
+/* A paged int8 cache: page p, KV head h holds rows [page_size][head_dim] of
+ * codes at ((p * n_kv_heads + h) * page_size) * head_dim, in K and in V, and one
+ * scale each at p * n_kv_heads + h; a code c stands for c * scale. */
+typedef struct wl_kv_pages_i8 {
+    int8_t *k, *v;             /* device, 16-byte aligned */
+    float *k_scale, *v_scale;  /* device */
+    uint32_t n_pages;
+    uint32_t page_size;        /* tokens: 16, 32, 64 or 128 */
+    uint32_t n_kv_heads, head_dim;
+} wl_kv_pages_i8;
+
+#define WL_ROPE_HALF 0u        /* pairs (j, j + n_rot / 2): the BitNet engine's */
+#define WL_ROPE_INTERLEAVED 1u /* pairs (2j, 2j + 1): the Llama engine's */
+
+/* Rotate q and k to their positions and append k and v to the cache.
+ * Sequence s owns tokens [seq_start[s], seq_start[s + 1]) of the call, at
+ * positions position[s], position[s] + 1, ...; position i lies in page
+ * page_table[s * max_pages + i / page_size], row i % page_size.  A call that
+ * writes a page's row 0 begins the page anew: its scale is (largest new
+ * |value|) / 127.  A page that earlier calls began keeps its scale while the
+ * new values fit and is doubled as often as they need otherwise; the codes in
+ * front of the new ones are then rounded again to the doubled steps.  So a
+ * value's code is off by at most half a step of the scale that it was written
+ * with, and by less than one step of the page's last scale.  Rows behind the
+ * new ones are left as they are.  NaN or infinity among a page's new values
+ * makes its scale NaN.
+ * rope: [rope_len][n_rot / 2] pairs (cos, sin), one row per position (any
+ * frequency scaling is the table's); elements from n_rot on are not rotated;
+ * n_rot 0: none (rope may be NULL).  Products and sums are rounded to f32 one
+ * by one, as in the engines.
+ * q_out [n_tokens][n_q_heads * head_dim] takes the rotated queries, k_out and
+ * v_out [n_tokens][n_kv_heads * head_dim] (NULL: none) the rotated keys and the
+ * values as they were before quantisation, for wl_dev_attn_prompt: dense,
+ * rounded once to out_type; they must not overlap q, k or v.  q and q_out may
+ * both be NULL.
+ * A page may be written for one sequence only in a call, and calls on one
+ * cache must not overlap on the GPU. */
+typedef struct wl_kv_append {
+    const void *q, *k, *v;     /* device, type `type` */
+    uint64_t q_stride, k_stride, v_stride; /* elements between tokens */
+    const int32_t *seq_start;  /* device, n_seqs + 1, ascending from 0 */
+    const int32_t *position;   /* device, n_seqs: tokens in the cache before the call */
+    const int32_t *page_table; /* device, n_seqs x max_pages */
+    const float *rope;         /* device, 8-byte aligned */
+    void *q_out, *k_out, *v_out;
+    uint32_t type, out_type;   /* WL_GGML_F32, WL_GGML_F16 or WL_GGML_BF16 */
+    uint32_t n_tokens, n_seqs, n_q_heads, max_pages;
+    uint32_t n_rot, rope_len;
+    uint32_t rope_pairs;       /* WL_ROPE_HALF or WL_ROPE_INTERLEAVED */
+} wl_kv_append;
+int wl_dev_rope_kv_append_i8(const wl_kv_pages_i8 *cache, const wl_kv_append *args, void *stream);
+
+/* Attention of one token per sequence over its first length[s] positions of
+ * the cache: out = softmax(scale * q . k) v for each query head, zeros where
+ * length[s] is 0.  Softmax and sums in f32.  workspace:
+ * wl_attn_decode_workspace_bytes bytes, 16-byte aligned, zero before the first
+ * call; every call leaves its counters zero again.  Calls that share a
+ * workspace must not overlap on the GPU (graphs replayed side by side each
+ * need their own). */
+typedef struct wl_attn_decode {
+    const void *q;             /* device: sequence s at s * q_stride */
+    void *out;                 /* device: sequence s at s * out_stride */
+    uint64_t q_stride, out_stride;
+    const int32_t *length;     /* device, n_seqs */
+    const int32_t *page_table; /* device, n_seqs x max_pages */
+    void *workspace;
+    size_t workspace_bytes;
+    uint32_t type, out_type;   /* of q / out: WL_GGML_F32, WL_GGML_F16 or WL_GGML_BF16 */
+    uint32_t n_seqs, n_q_heads, max_pages;
+    float scale;
+} wl_attn_decode;
+size_t wl_attn_decode_workspace_bytes(uint32_t n_seqs, uint32_t n_q_heads, uint32_t n_kv_heads,
+                                      uint32_t head_dim);
+int wl_dev_attn_decode_i8(const wl_kv_pages_i8 *cache, const wl_attn_decode *args, void *stream);
+
+/* Causal attention within packed prompts: row i of sequence s (rows
+ * seq_start[s] .. seq_start[s + 1] of q, k, v) attends to rows 0 .. i of the
+ * same sequence.  What masked rows hold, NaN included, has no effect.  Rows
+ * of out that no sequence owns are left as they were.  q, k and v are all
+ * WL_GGML_F16 or all WL_GGML_BF16; out is that type or WL_GGML_F32.  Scores,
+ * softmax and sums in f32; the weights enter the product with v in the
+ * inputs' 16-bit type.  out must not overlap q, k or v. */
+typedef struct wl_attn_prompt {
+    const void *q, *k, *v;     /* device */
+    void *out;                 /* device */
+    uint64_t q_stride, k_stride, v_stride, out_stride; /* elements between tokens */
+    const int32_t *seq_start;  /* device, n_seqs + 1, ascending from 0 */
+    uint32_t type, out_type;
+    uint32_t n_tokens, n_seqs, n_q_heads, n_kv_heads, head_dim;
+    float scale;
+} wl_attn_prompt;
+int wl_dev_attn_prompt(const wl_attn_prompt *args, void *stream);
 
 /* ------------------------------------------------ tensor parallel (one GPU per process)
  * North star: BitLinear output rows split across the GPUs of one box with an

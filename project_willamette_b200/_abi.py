@@ -103,6 +103,41 @@ class WlLlamaWeights(C.Structure):
                 ("token_embd", C.c_void_p)]
 
 
+WL_GGML_BF16 = 30
+WL_ROPE_HALF = 0         # pairs (j, j + n_rot / 2)
+WL_ROPE_INTERLEAVED = 1  # pairs (2j, 2j + 1)
+
+
+class WlKvPagesI8(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + \
+               [(n, C.c_uint32) for n in ("n_pages", "page_size", "n_kv_heads", "head_dim")]
+
+
+class WlKvAppend(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v")] + \
+               [(n, C.c_uint64) for n in ("q_stride", "k_stride", "v_stride")] + \
+               [(n, C.c_void_p) for n in ("seq_start", "position", "page_table", "rope", "q_out",
+                                          "k_out", "v_out")] + \
+               [(n, C.c_uint32) for n in ("type", "out_type", "n_tokens", "n_seqs", "n_q_heads",
+                                          "max_pages", "n_rot", "rope_len", "rope_pairs")]
+
+
+class WlAttnDecode(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_uint64),
+                ("out_stride", C.c_uint64), ("length", C.c_void_p), ("page_table", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)] + \
+               [(n, C.c_uint32) for n in ("type", "out_type", "n_seqs", "n_q_heads",
+                                          "max_pages")] + [("scale", C.c_float)]
+
+
+class WlAttnPrompt(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out")] + \
+               [(n, C.c_uint64) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] + \
+               [("seq_start", C.c_void_p)] + \
+               [(n, C.c_uint32) for n in ("type", "out_type", "n_tokens", "n_seqs", "n_q_heads",
+                                          "n_kv_heads", "head_dim")] + [("scale", C.c_float)]
+
+
 _vp = C.c_void_p
 _sz = C.c_size_t
 _u32 = C.c_uint32
@@ -152,6 +187,10 @@ PROTOTYPES = {
     "wl_q8_0_packed_bytes": ([_u32, _u32], _sz),
     "wl_dev_q8_0_repack": ([_vp, _u32, _u32, _vp, _vp], _i),
     "wl_dev_q8_0_matvec": ([_vp, _u32, _u32, _vp, _vp, _vp], _i),
+    "wl_dev_rope_kv_append_i8": ([C.POINTER(WlKvPagesI8), C.POINTER(WlKvAppend), _vp], _i),
+    "wl_attn_decode_workspace_bytes": ([_u32, _u32, _u32, _u32], _sz),
+    "wl_dev_attn_decode_i8": ([C.POINTER(WlKvPagesI8), C.POINTER(WlAttnDecode), _vp], _i),
+    "wl_dev_attn_prompt": ([C.POINTER(WlAttnPrompt), _vp], _i),
     "wl_bitnet_create": ([C.POINTER(WlBitnetConfig), C.POINTER(WlBitnetWeights), C.POINTER(_vp)],
                          _i),
     "wl_bitnet_create_tp": ([C.POINTER(WlBitnetConfig), C.POINTER(WlBitnetWeights), _vp,

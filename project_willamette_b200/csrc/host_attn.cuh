@@ -1,0 +1,295 @@
+// host_attn.cuh -- host side of the attention operators over caller buffers:
+// argument checks and launches of the paged int8 KV append, the decode
+// attention over that cache and the packed prompt attention.
+//
+// Part of the library's single translation unit (see host_core.cuh).
+#pragma once
+
+namespace {
+
+// WL_GGML_* of an activation buffer -> the kernels' type index, or -1.
+int act_type(uint32_t ggml) {
+    return ggml == WL_GGML_F32 ? 0 : ggml == WL_GGML_F16 ? 1 : ggml == WL_GGML_BF16 ? 2 : -1;
+}
+uint64_t act_size(int type) { return type == 0 ? 4u : 2u; }
+
+// A buffer of rows with `stride` elements between tokens and `width` elements
+// used of each: 16-byte aligned rows that do not run into one another.
+int check_rows(const char *op, const char *name, const void *p, uint64_t stride, uint64_t width,
+               int type) {
+    if (!p) return fail(WL_ERR_INVALID_ARGUMENT, "%s: %s is NULL", op, name);
+    if (!aligned16(p))
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: %s is not 16-byte aligned", op, name);
+    if (stride < width || stride > (1ull << 31) || stride * act_size(type) % 16u)
+        return fail(WL_ERR_INVALID_ARGUMENT,
+                    "%s: %s stride %llu must be at least its %llu elements, at most 2^31, and a "
+                    "multiple of 16 bytes",
+                    op, name, (unsigned long long)stride, (unsigned long long)width);
+    return WL_OK;
+}
+
+int check_i32(const char *op, const char *name, const int32_t *p) {
+    if (!p || (reinterpret_cast<uintptr_t>(p) & 3u))
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: %s is NULL or not 4-byte aligned", op, name);
+    return WL_OK;
+}
+
+int check_heads(const char *op, uint32_t n_q, uint32_t n_kv, uint32_t head_dim) {
+    if (head_dim != 64 && head_dim != 128)
+        return fail(WL_ERR_NOT_IMPLEMENTED, "%s: head_dim %u is neither 64 nor 128", op, head_dim);
+    if (!n_kv || !n_q || n_q % n_kv || n_kv > 1024 || n_q > 65535)
+        return fail(WL_ERR_INVALID_ARGUMENT,
+                    "%s: %u query heads over %u KV heads (a positive multiple, at most 1024 KV and "
+                    "65535 query heads)",
+                    op, n_q, n_kv);
+    return WL_OK;
+}
+
+int check_kv_pages(const char *op, const wl_kv_pages_i8 *c) {
+    if (!c) return fail(WL_ERR_INVALID_ARGUMENT, "%s: cache is NULL", op);
+    if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128)
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: page_size %u is not 16, 32, 64 or 128", op,
+                    c->page_size);
+    if (!c->k || !c->v || !aligned16(c->k) || !aligned16(c->v))
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: k / v pages NULL or not 16-byte aligned", op);
+    if (!c->k_scale || !c->v_scale || (reinterpret_cast<uintptr_t>(c->k_scale) & 3u) ||
+        (reinterpret_cast<uintptr_t>(c->v_scale) & 3u))
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: page scales NULL or not 4-byte aligned", op);
+    if (!c->n_pages || c->n_pages > 0x7FFFFFFFu)
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: %u pages", op, c->n_pages);
+    return WL_OK;
+}
+
+// Where these operators report a bad index read on the device: the second
+// word of the library's status block, so that a bad index is not taken for a
+// timed-out wait by the host-buffer calls, which read the first.
+int attn_status(const char *op, uint32_t **status) {
+    uint32_t *s = status_ptr();
+    if (!s) return WL_ERR_NO_DEVICE;
+    int dev = -1;
+    WL_CUDA(cudaGetDevice(&dev));
+    if (dev != ctx().device)
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: the current device is %d, the library runs on %d",
+                    op, dev, ctx().device);
+    *status = s + 1;
+    return WL_OK;
+}
+
+template <typename T>
+int launch_kv_append(const KvAppendParams &p, dim3 grid, cudaStream_t s) {
+    const uint32_t pieces = p.page_size * p.head_dim / 8u;  // 8-element pieces of a page and head
+    if (pieces <= 128)
+        WL_CUDA(launch(kv_append_kernel<T, 1, 128>, grid, dim3(256), 0, s, true, p));
+    else if (pieces <= 256)
+        WL_CUDA(launch(kv_append_kernel<T, 2, 128>, grid, dim3(256), 0, s, true, p));
+    else if (pieces <= 512)
+        WL_CUDA(launch(kv_append_kernel<T, 4, 128>, grid, dim3(256), 0, s, true, p));
+    else if (pieces <= 1024)
+        WL_CUDA(launch(kv_append_kernel<T, 8, 128>, grid, dim3(256), 0, s, true, p));
+    else
+        WL_CUDA(launch(kv_append_kernel<T, 8, 256>, grid, dim3(512), 0, s, true, p));
+    return WL_OK;
+}
+
+template <typename T>
+int launch_attn_prompt(const AttnPromptParams &p, uint32_t head_dim, cudaStream_t s) {
+    const dim3 grid((p.n_tokens + 3u) / 4u, p.group * p.n_kv);
+    if (head_dim == 64)
+        WL_CUDA(launch(attn_prompt_rows_kernel<T, 64>, grid, dim3(128), 0, s, true, p));
+    else
+        WL_CUDA(launch(attn_prompt_rows_kernel<T, 128>, grid, dim3(128), 0, s, true, p));
+    return WL_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int wl_dev_rope_kv_append_i8(const wl_kv_pages_i8 *cache, const wl_kv_append *a, void *stream) {
+    const char *op = "rope_kv_append";
+    int rc = check_kv_pages(op, cache);
+    if (rc) return rc;
+    if (!a) return fail(WL_ERR_INVALID_ARGUMENT, "%s: args is NULL", op);
+    const uint32_t D = cache->head_dim, KV = cache->n_kv_heads;
+    const uint32_t n_q = a->q ? a->n_q_heads : KV;
+    if ((rc = check_heads(op, n_q, KV, D))) return rc;
+    const int type = act_type(a->type), out_type = act_type(a->out_type);
+    if (type < 0) return fail_type(a->type);
+    if (out_type < 0) return fail_type(a->out_type);
+    if (a->n_rot % 2 || a->n_rot > D)
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: n_rot %u must be even and at most %u", op,
+                    a->n_rot, D);
+    if (a->rope_pairs > 1)
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: rope_pairs %u is neither WL_ROPE_HALF nor "
+                    "WL_ROPE_INTERLEAVED", op, a->rope_pairs);
+    if (a->n_tokens > 0x7FFFFFFFu || a->n_seqs > 0x3FFFFFFFu)
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: %u tokens of %u sequences", op, a->n_tokens,
+                    a->n_seqs);
+    if (a->n_tokens == 0 || a->n_seqs == 0) return WL_OK;
+    if ((rc = check_rows(op, "k", a->k, a->k_stride, (uint64_t)KV * D, type)) ||
+        (rc = check_rows(op, "v", a->v, a->v_stride, (uint64_t)KV * D, type)) ||
+        (a->q && (rc = check_rows(op, "q", a->q, a->q_stride, (uint64_t)n_q * D, type))) ||
+        (rc = check_i32(op, "seq_start", a->seq_start)) ||
+        (rc = check_i32(op, "position", a->position)) ||
+        (rc = check_i32(op, "page_table", a->page_table)))
+        return rc;
+    if (!a->q != !a->q_out)
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: q and q_out go together", op);
+    if (!aligned16(a->q_out) || !aligned16(a->k_out) || !aligned16(a->v_out))
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: q_out / k_out / v_out not 16-byte aligned", op);
+    if (a->n_rot && (!a->rope || (reinterpret_cast<uintptr_t>(a->rope) & 7u)))
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: rope is NULL or not 8-byte aligned", op);
+    if (a->max_pages == 0 || a->max_pages > 0x7FFFFFFFu / cache->page_size)
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: max_pages %u", op, a->max_pages);
+    KvAppendParams p;
+    memset(&p, 0, sizeof p);
+    if ((rc = attn_status(op, &p.status))) return rc;
+    p.kc = cache->k;
+    p.vc = cache->v;
+    p.ks = cache->k_scale;
+    p.vs = cache->v_scale;
+    p.n_pages = cache->n_pages;
+    p.page_size = cache->page_size;
+    p.n_kv = KV;
+    p.head_dim = D;
+    p.q = a->q;
+    p.k = a->k;
+    p.v = a->v;
+    p.q_stride = a->q_stride;
+    p.k_stride = a->k_stride;
+    p.v_stride = a->v_stride;
+    p.seq_start = a->seq_start;
+    p.position = a->position;
+    p.page_table = a->page_table;
+    p.rope = reinterpret_cast<const float2 *>(a->rope);
+    p.q_out = a->q_out;
+    p.k_out = a->k_out;
+    p.v_out = a->v_out;
+    p.out_type = (uint32_t)out_type;
+    p.n_tokens = a->n_tokens;
+    p.n_seqs = a->n_seqs;
+    p.group = n_q / KV;
+    p.max_pages = a->max_pages;
+    p.n_rot = a->n_rot;
+    p.rope_len = a->rope_len;
+    p.rope_pairs = a->rope_pairs;
+    const uint64_t units = (uint64_t)a->n_tokens / cache->page_size + 2ull * a->n_seqs;
+    if (units > 0x7FFFFFFFull)
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: %u tokens of %u sequences", op, a->n_tokens,
+                    a->n_seqs);
+    const dim3 grid((uint32_t)units, KV);
+    if (type == 0) return launch_kv_append<float>(p, grid, (cudaStream_t)stream);
+    if (type == 1) return launch_kv_append<__half>(p, grid, (cudaStream_t)stream);
+    return launch_kv_append<__nv_bfloat16>(p, grid, (cudaStream_t)stream);
+}
+
+size_t wl_attn_decode_workspace_bytes(uint32_t n_seqs, uint32_t n_q_heads, uint32_t n_kv_heads,
+                                      uint32_t head_dim) {
+    (void)n_seqs;
+    (void)n_q_heads;
+    (void)n_kv_heads;
+    (void)head_dim;
+    return 16;
+}
+
+int wl_dev_attn_decode_i8(const wl_kv_pages_i8 *cache, const wl_attn_decode *a, void *stream) {
+    const char *op = "attn_decode";
+    int rc = check_kv_pages(op, cache);
+    if (rc) return rc;
+    if (!a) return fail(WL_ERR_INVALID_ARGUMENT, "%s: args is NULL", op);
+    const uint32_t D = cache->head_dim, KV = cache->n_kv_heads;
+    if ((rc = check_heads(op, a->n_q_heads, KV, D))) return rc;
+    const int type = act_type(a->type), out_type = act_type(a->out_type);
+    if (type < 0) return fail_type(a->type);
+    if (out_type < 0) return fail_type(a->out_type);
+    if (!std::isfinite(a->scale))
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: scale is not finite", op);
+    if (a->n_seqs > 65535)
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: %u sequences (at most 65535)", op, a->n_seqs);
+    if (a->n_seqs == 0) return WL_OK;
+    const uint64_t width = (uint64_t)a->n_q_heads * D;
+    if ((rc = check_rows(op, "q", a->q, a->q_stride, width, type)) ||
+        (rc = check_rows(op, "out", a->out, a->out_stride, width, out_type)) ||
+        (rc = check_i32(op, "length", a->length)) ||
+        (rc = check_i32(op, "page_table", a->page_table)))
+        return rc;
+    if (a->max_pages == 0 || a->max_pages > 0x7FFFFFFFu / cache->page_size)
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: max_pages %u", op, a->max_pages);
+    const size_t need = wl_attn_decode_workspace_bytes(a->n_seqs, a->n_q_heads, KV, D);
+    if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < need)
+        return fail(WL_ERR_INVALID_ARGUMENT,
+                    "%s: workspace NULL, not 16-byte aligned, or smaller than "
+                    "wl_attn_decode_workspace_bytes (%zu)",
+                    op, need);
+    AttnDecodeParams p;
+    memset(&p, 0, sizeof p);
+    if ((rc = attn_status(op, &p.status))) return rc;
+    p.kc = cache->k;
+    p.vc = cache->v;
+    p.ks = cache->k_scale;
+    p.vs = cache->v_scale;
+    p.n_pages = cache->n_pages;
+    p.page_size = cache->page_size;
+    p.n_kv = KV;
+    p.head_dim = D;
+    p.q = a->q;
+    p.out = a->out;
+    p.q_stride = a->q_stride;
+    p.out_stride = a->out_stride;
+    p.length = a->length;
+    p.page_table = a->page_table;
+    p.type = (uint32_t)type;
+    p.out_type = (uint32_t)out_type;
+    p.n_seqs = a->n_seqs;
+    p.group = a->n_q_heads / KV;
+    p.max_pages = a->max_pages;
+    p.scale = a->scale;
+    WL_CUDA(launch(attn_decode_i8_kernel, dim3(a->n_q_heads, a->n_seqs), dim3(PAGED_THREADS), 0,
+                   (cudaStream_t)stream, true, p));
+    return WL_OK;
+}
+
+int wl_dev_attn_prompt(const wl_attn_prompt *a, void *stream) {
+    const char *op = "attn_prompt";
+    if (!a) return fail(WL_ERR_INVALID_ARGUMENT, "%s: args is NULL", op);
+    const uint32_t D = a->head_dim, H = a->n_q_heads, KV = a->n_kv_heads;
+    int rc = check_heads(op, H, KV, D);
+    if (rc) return rc;
+    const int type = act_type(a->type), out_type = act_type(a->out_type);
+    if (type < 1) return fail_type(a->type);
+    if (out_type < 0 || (out_type && out_type != type)) return fail_type(a->out_type);
+    if (!std::isfinite(a->scale))
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: scale is not finite", op);
+    if (a->n_tokens > 0x7FFFFFFFu || a->n_seqs > 0x3FFFFFFFu)
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: %u tokens of %u sequences", op, a->n_tokens,
+                    a->n_seqs);
+    if (a->n_tokens == 0 || a->n_seqs == 0) return WL_OK;
+    if ((rc = check_rows(op, "q", a->q, a->q_stride, (uint64_t)H * D, type)) ||
+        (rc = check_rows(op, "k", a->k, a->k_stride, (uint64_t)KV * D, type)) ||
+        (rc = check_rows(op, "v", a->v, a->v_stride, (uint64_t)KV * D, type)) ||
+        (rc = check_rows(op, "out", a->out, a->out_stride, (uint64_t)H * D, out_type)) ||
+        (rc = check_i32(op, "seq_start", a->seq_start)))
+        return rc;
+    AttnPromptParams p;
+    memset(&p, 0, sizeof p);
+    if ((rc = attn_status(op, &p.status))) return rc;
+    p.q = a->q;
+    p.k = a->k;
+    p.v = a->v;
+    p.out = a->out;
+    p.q_stride = a->q_stride;
+    p.k_stride = a->k_stride;
+    p.v_stride = a->v_stride;
+    p.out_stride = a->out_stride;
+    p.seq_start = a->seq_start;
+    p.out_type = (uint32_t)out_type;
+    p.n_tokens = a->n_tokens;
+    p.n_seqs = a->n_seqs;
+    p.group = H / KV;
+    p.n_kv = KV;
+    p.scale = a->scale;
+    if (type == 1) return launch_attn_prompt<__half>(p, D, (cudaStream_t)stream);
+    return launch_attn_prompt<__nv_bfloat16>(p, D, (cudaStream_t)stream);
+}
+
+}  // extern "C"

@@ -8,6 +8,7 @@
 //   host_bitnet.cuh  BitNet decode engine (wl_bitnet_*)
 //   host_llama.cuh   batched Q8_0 Llama decode engine (wl_llama_batch_*)
 //   host_gguf.cuh    GGUF model configuration and engine upload
+//   host_attn.cuh    paged int8 KV append, decode and prompt attention
 // Built as one translation unit with the kernel headers so the whole library
 // is a single sm_100a object (see project_willamette_b200/build.py).
 #include <cuda_runtime.h>
@@ -35,6 +36,9 @@
 #include "q8_0.cuh"
 #include "q8_batch.cuh"
 #include "attn_batch.cuh"
+#include "kv_append.cuh"
+#include "attn_paged.cuh"
+#include "attn_prompt.cuh"
 #include "gguf.h"
 
 #include "host_core.cuh"
@@ -89,13 +93,13 @@ int wl_device_status(uint32_t *flags) {
     }
     rc = ensure_init(c);
     if (rc) return rc;
-    uint32_t f = 0;
+    uint32_t f[2] = {0, 0};  // waits | indexes of the attention operators
     // Kernels of every stream (library and caller streams) must have finished.
     WL_CUDA(cudaDeviceSynchronize());
-    WL_CUDA(cudaMemcpy(&f, c.d_status, 4, cudaMemcpyDeviceToHost));
-    WL_CUDA(cudaMemset(c.d_status, 0, 4));
+    WL_CUDA(cudaMemcpy(f, c.d_status, 8, cudaMemcpyDeviceToHost));
+    WL_CUDA(cudaMemset(c.d_status, 0, 8));
     WL_CUDA(cudaDeviceSynchronize());
-    if (flags) *flags = f | na;
+    if (flags) *flags = f[0] | f[1] | na;
     return WL_OK;
 }
 
@@ -620,3 +624,4 @@ int wl_dev_i2s_gemm_s8_f32(const int8_t *ternary, float w_scale, uint32_t in_dim
 #include "host_bitnet.cuh"
 #include "host_llama.cuh"
 #include "host_gguf.cuh"
+#include "host_attn.cuh"
