@@ -185,11 +185,11 @@ int wl_dev_rope_kv_append_i8(const wl_kv_pages_i8 *cache, const wl_kv_append *a,
 
 size_t wl_attn_decode_workspace_bytes(uint32_t n_seqs, uint32_t n_q_heads, uint32_t n_kv_heads,
                                       uint32_t head_dim) {
+    // one size serves every batch: it follows the GPU's CTAs, not the sequences
     (void)n_seqs;
     (void)n_q_heads;
     (void)n_kv_heads;
-    (void)head_dim;
-    return 16;
+    return paged_workspace_bytes(head_dim);
 }
 
 int wl_dev_attn_decode_i8(const wl_kv_pages_i8 *cache, const wl_attn_decode *a, void *stream) {
@@ -244,8 +244,15 @@ int wl_dev_attn_decode_i8(const wl_kv_pages_i8 *cache, const wl_attn_decode *a, 
     p.group = a->n_q_heads / KV;
     p.max_pages = a->max_pages;
     p.scale = a->scale;
-    WL_CUDA(launch(attn_decode_i8_kernel, dim3(a->n_q_heads, a->n_seqs), dim3(PAGED_THREADS), 0,
-                   (cudaStream_t)stream, true, p));
+    p.workspace = a->workspace;
+    const uint32_t ctas = std::min<uint32_t>((uint32_t)sm_count_for_launch() * PAGED_CTAS_PER_SM,
+                                             PAGED_MAX_CTAS);
+    if (D == 64)
+        WL_CUDA(launch(attn_decode_i8_kernel<64>, dim3(ctas), dim3(PAGED_THREADS), 0,
+                       (cudaStream_t)stream, true, p));
+    else
+        WL_CUDA(launch(attn_decode_i8_kernel<128>, dim3(ctas), dim3(PAGED_THREADS), 0,
+                       (cudaStream_t)stream, true, p));
     return WL_OK;
 }
 

@@ -203,7 +203,10 @@ def decode_ref(cache, q, length, table, heads, scale):
     exponent, twice (once in the sum below the line): the dot product's dim + 4 roundings of
     2^-24, relative to scale * |q| . |k| (a split of q in two 16-bit parts has 22 bits and counts as
     four more), plus 2^-20 for exp, exponent and scale products; the sums over keys by one
-    rounding per key."""
+    rounding per key.  A weight also has an absolute error: as e^(z - m) * 2^14, at most 2^14, it is
+    split into two f16 numbers whose remainder is at most half of f16's smallest, 2^-25, so 2^-39
+    of the largest weight, which is 1 before the division by a sum of at least 1; it multiplies
+    |code| and, since weights are taken relative to it, the largest scale."""
     S, G, D = q.shape[0], heads // cache.kv, cache.dim
     out = torch.zeros(S, heads, D, dtype=torch.float64, device="cuda")
     tol = torch.zeros_like(out)
@@ -220,6 +223,8 @@ def decode_ref(cache, q, length, table, heads, scale):
             size = (x.abs() @ k.abs().T * abs(scale)).amax(-1, keepdim=True)
             out[i, h * G:(h + 1) * G], a = softmax_rows(z, v)
             tol[i, h * G:(h + 1) * G] = a * (2 * (size * (D + 8) * 2.0 ** -24 + 2.0 ** -20) + (n + 64) * 2.0 ** -24)
+            c_abs = cache.v[pages, h].double().abs().reshape(-1, D)[:n].sum(0)
+            tol[i, h * G:(h + 1) * G] += 2.0 ** -39 * cache.vs[pages, h].double().max() * c_abs
     return out.flatten(1), tol.flatten(1)
 
 
