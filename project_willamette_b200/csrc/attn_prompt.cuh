@@ -7,9 +7,12 @@
 // Rows outside every sequence are left as they were.
 #pragma once
 
+#include <cuda.h>
+
 #include <cstdint>
 
 #include "attn_paged.cuh"
+#include "i2s_gemm.cuh"
 
 namespace wl {
 
@@ -80,22 +83,399 @@ __device__ __forceinline__ void prompt_row(const AttnPromptParams &p, int64_t be
                     acc[i] / l);
 }
 
-// One warp per (row, head).
+// ------------------------------------------------------------------ tensor cores
+// A CTA takes 256 rows of one head as two tiles of 128, and goes through the
+// keys 128 at a time.  Tensor memory (512 columns): scores of both tiles (128
+// f32 columns each; the weights overwrite them as 16-bit pairs) and both
+// outputs (D f32 columns each).
+//   warps 0-3, 4-7  softmax of tile 0 / 1, one thread a row: scores to
+//                   registers, row maximum, weights 2^(z - m + 6) back as 16-bit;
+//                   the output is rescaled only when the maximum has risen by more
+//                   than 2^8 over the one in use (weights then stay below 2^14);
+//   warp 8          TMA: queries, then keys and values through a ring;
+//   warp 9          MMA (one thread): weights x values of step j, then queries x keys
+//                   of step j + 1, for one tile and the other in turn, so that one
+//                   tile's softmax runs beside the other tile's products.
+// A commit on the scores of step j + 1 covers the earlier product into the
+// output as well, so who reads those scores may also rescale the output.
+// The masked part of a product is 0 x v, which is NaN where v is not finite:
+// a row whose output is not finite is computed again by prompt_row, which does
+// not read what the mask leaves out.
+constexpr int PROMPT_THREADS = 320;
+constexpr int PROMPT_ROWS = 256;
+
+template <int D>
+struct PromptSmem {
+    static constexpr uint32_t TILE = 128u * D * 2u;      // 128 rows of queries, keys or values
+    static constexpr uint32_t STAGES = D == 128 ? 5 : 8;
+    static constexpr size_t DYN = (2 + STAGES) * TILE + 1024;  // + alignment slack
+};
+
+struct AttnPromptMaps {
+    CUtensorMap q, k, v;  // [token][head][D] 16-bit, box {64, 1, 128}, 128-byte swizzle
+};
+
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint32_t x, uint32_t y,
+                                            uint32_t z, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// D f32, A and B both f16 or both bf16, M = 128; b_mn: B is stored with its N
+// dimension contiguous (values), not K (keys).
+__device__ __forceinline__ uint32_t umma_idesc_f16(uint32_t bf16, uint32_t b_mn, uint32_t n) {
+    return (1u << 4) | (bf16 << 7) | (bf16 << 10) | (b_mn << 16) | ((n >> 3) << 17) | (8u << 24);
+}
+// Operand stored [k][64 n] with 128-byte rows, 128-byte swizzle: groups of 8 k are
+// 1024 bytes apart, blocks of 64 n `block` bytes.
+__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr, uint32_t block) {
+    return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | ((uint64_t)(block >> 4) << 16) |
+           ((uint64_t)(1024u >> 4) << 32) | ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
+}
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                            uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                            uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+#define WL_R8(r, i)                                                                          \
+    "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), \
+        "=r"(r[i + 6]), "=r"(r[i + 7])
+#define WL_IN8(r, i)                                                                      \
+    "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), \
+        "r"(r[i + 6]), "r"(r[i + 7])
+// 32 columns of this warp's 32 lanes; the caller waits (tmem_wait_ld).
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : WL_R8(r, 0), WL_R8(r, 8), WL_R8(r, 16), WL_R8(r, 24)
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::WL_IN8(r, 0),
+        WL_IN8(r, 8), WL_IN8(r, 16), WL_IN8(r, 24), "r"(taddr)
+        : "memory");
+}
+#undef WL_R8
+#undef WL_IN8
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack16<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(128) attn_prompt_rows_kernel(const AttnPromptParams p) {
+__global__ void __launch_bounds__(PROMPT_THREADS, 1)
+    attn_prompt_kernel(const __grid_constant__ AttnPromptMaps maps, const AttnPromptParams p) {
+    using L = PromptSmem<D>;
+    constexpr uint32_t ST = L::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t q_full[2], kv_full[ST], kv_empty[ST], s_full[2], p_full[2], o_full[2];
+    __shared__ uint32_t s_tmem, s_abort, s_seq;
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                                ~(uintptr_t)1023);
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    // longest rows first: units in descending order, heads side by side
+    const uint32_t heads = p.n_kv * p.group, head = blockIdx.x % heads;
+    const uint32_t unit = (gridDim.x - 1u - blockIdx.x) / heads;
+
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(&s_tmem)),
+                     "r"(512u));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&q_full[i], 1);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);  // one arrival a softmax warp
+            mbar_init(&o_full[i], 1);
+        }
+        for (uint32_t s = 0; s < ST; ++s) {
+            mbar_init(&kv_full[s], 1);
+            mbar_init(&kv_empty[s], 1);
+        }
+        s_abort = 0;
+        fence_mbar_init();
+    }
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t lane = threadIdx.x & 31u;
-    const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 32u;
-    if (row >= p.n_tokens) return;
-    const uint32_t seq = find_seq(p.seq_start, p.n_seqs, 1u, 0u, (uint32_t)row, lane);
-    const int64_t begin = __ldg(p.seq_start + seq), end = __ldg(p.seq_start + seq + 1);
-    if (begin < 0 || end < begin || end > (int64_t)p.n_tokens) {
-        if (lane == 0) atomicOr(p.status, WL_DEV_ERR_INDEX);
-        return;
+    if (warp == 8) {
+        const uint32_t s = find_seq(p.seq_start, p.n_seqs, PROMPT_ROWS, 1u, unit, lane);
+        if (lane == 0) s_seq = s;
     }
-    if (row < begin || row >= end) return;
-    prompt_row<T, D>(p, begin, row, blockIdx.y, lane);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+
+    // this CTA's rows: [row0, row0 + 256) of the sequence, where there are any
+    const uint32_t seq = s_seq;
+    const int64_t begin = __ldg(p.seq_start + seq), stop = __ldg(p.seq_start + seq + 1);
+    const bool bad = begin < 0 || stop < begin || stop > (int64_t)p.n_tokens;
+    if (bad && tid == 0) atomicOr(p.status, WL_DEV_ERR_INDEX);
+    const int64_t len = stop - begin;
+    const int64_t row0 = ((int64_t)unit - (begin / PROMPT_ROWS + (int64_t)seq)) * PROMPT_ROWS;
+    uint32_t steps[2] = {0u, 0u};  // 128-key steps of each tile
+    if (!bad && row0 >= 0) {
+        if (row0 < len) steps[0] = (uint32_t)(row0 / 128) + 1u;
+        if (row0 + 128 < len) steps[1] = steps[0] + 1u;
+    }
+    const uint32_t n_steps = max(steps[0], steps[1]);
+
+    auto aborted = [&]() { return *(volatile uint32_t *)&s_abort != 0u; };
+    auto wait = [&](uint64_t *bar, uint32_t parity) {  // false: the wait ran out, here or elsewhere
+        if (mbar_try_wait(bar, parity)) return true;
+        const uint64_t t0 = globaltimer_ns(), limit = wait_limit_ns();
+        while (!mbar_try_wait(bar, parity)) {
+            if (aborted()) return false;
+            if (globaltimer_ns() - t0 > limit) {
+                atomicOr(p.status - 1, WL_DEV_ERR_TIMEOUT);
+                atomicExch(&s_abort, 1u);
+                return false;
+            }
+        }
+        return true;
+    };
+
+    if (warp == 8) {
+        if (lane == 0 && n_steps) {
+            const uint32_t h = head / p.group, z0 = (uint32_t)(begin + row0);
+            auto load_tile = [&](uint8_t *dst, const CUtensorMap *map, uint32_t y, uint32_t z, uint64_t *bar) {
+                mbar_arrive_expect_tx(bar, L::TILE);
+#pragma unroll
+                for (uint32_t x = 0; x < (uint32_t)D; x += 64) tma_load_3d(dst + x * 256u, map, x, y, z, bar);
+            };
+            uint32_t it = 0;
+            auto load_kv = [&](const CUtensorMap *map, uint32_t j) {
+                const uint32_t s = it % ST;
+                if (it >= ST && !wait(&kv_empty[s], (it / ST - 1u) & 1u)) return false;
+                load_tile(smem + (2u + s) * L::TILE, map, h, (uint32_t)begin + j * 128u, &kv_full[s]);
+                ++it;
+                return true;
+            };
+            load_tile(smem, &maps.q, head, z0, &q_full[0]);
+            bool ok = load_kv(&maps.k, 0);
+            if (steps[1]) load_tile(smem + L::TILE, &maps.q, head, z0 + 128u, &q_full[1]);
+            for (uint32_t j = 0; ok && j < n_steps; ++j) {
+                if (j) ok = load_kv(&maps.k, j);
+                if (ok) ok = load_kv(&maps.v, j);
+            }
+            // (bounded) the last copies land before the CTA's shared memory goes
+            (void)mbar_wait(&q_full[0], 0);
+            if (steps[1]) (void)mbar_wait(&q_full[1], 0);
+            for (uint32_t k = it > ST ? it - ST : 0; k < it; ++k)
+                (void)mbar_wait(&kv_full[k % ST], (k / ST) & 1u);
+        }
+    } else if (warp == 9) {
+        if (lane == 0 && n_steps) {
+            const uint32_t bf = sizeof(T) == 2 && pack16<T>(1.0f, 0.0f) == 0x3F80u;
+            const uint32_t idesc_s = umma_idesc_f16(bf, 0u, 128u), idesc_o = umma_idesc_f16(bf, 1u, D);
+            auto stage = [&](uint32_t it) { return smem_u32(smem + (2u + it % ST) * L::TILE); };
+            auto scores = [&](uint32_t t, uint32_t it) {  // tile t: S = Q K^T, keys of ring entry it
+                const uint32_t q = smem_u32(smem + t * L::TILE), k = stage(it);
+#pragma unroll
+                for (uint32_t i = 0; i < (uint32_t)D / 16; ++i) {
+                    const uint32_t off = (i / 4u) * 16384u + (i % 4u) * 32u;
+                    umma_f16_ss(tmem + t * 128u, umma_desc_sw128(q + off), umma_desc_sw128(k + off), idesc_s,
+                                i != 0u);
+                }
+                umma_commit(&s_full[t]);
+            };
+            auto outputs = [&](uint32_t t, uint32_t it, bool add) {  // tile t: O += W V
+                const uint32_t v = stage(it);
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i)
+                    umma_f16_ts(tmem + 256u + t * 128u, tmem + t * 128u + i * 8u,
+                                umma_desc_mn_sw128(v + i * 2048u, 16384u), idesc_o, add || i != 0u);
+            };
+            // ring entries: K0, V0, K1, V1, ...
+            bool ok = wait(&kv_full[0], 0);
+            uint32_t issued = 0;  // committed ring entries, for the drain
+            for (uint32_t t = 0; ok && t < 2; ++t) {
+                if (!steps[t]) continue;
+                if (!(ok = wait(&q_full[t], 0))) break;
+                tc_fence_after();
+                scores(t, 0);
+            }
+            if (ok) {
+                umma_commit(&kv_empty[0]);
+                issued = 1;
+            }
+            for (uint32_t j = 0; ok && j < n_steps; ++j) {
+                const uint32_t v = 2u * j + 1u, k = v + 1u;
+                if (!(ok = wait(&kv_full[v % ST], (v / ST) & 1u))) break;
+                if (j + 1 < n_steps && !(ok = wait(&kv_full[k % ST], (k / ST) & 1u))) break;
+                for (uint32_t t = 0; t < 2; ++t) {
+                    if (j >= steps[t]) continue;
+                    if (!(ok = wait(&p_full[t], j & 1u))) break;
+                    tc_fence_after();
+                    outputs(t, v, j != 0u);
+                    if (j + 1 < steps[t])
+                        scores(t, k);
+                    else
+                        umma_commit(&o_full[t]);
+                }
+                if (!ok) break;
+                umma_commit(&kv_empty[v % ST]);
+                issued = v + 1;
+                if (j + 1 < n_steps) {
+                    umma_commit(&kv_empty[k % ST]);
+                    issued = k + 1;
+                }
+            }
+            // (bounded) every committed product is done before tensor memory goes
+            for (uint32_t k = issued > ST ? issued - ST : 0; k < issued; ++k)
+                (void)mbar_wait(&kv_empty[k % ST], (k / ST) & 1u);
+        }
+    } else {
+        const uint32_t t = warp >> 2, r = (warp & 3u) * 32u + lane;  // tile, row in the tile
+        const uint32_t n = steps[t];
+        const uint32_t lanes = ((warp & 3u) * 32u) << 16;
+        const uint32_t ts = tmem + lanes + t * 128u, to = tmem + lanes + 256u + t * 128u;
+        const float sc = p.scale * 1.4426950408889634f;
+        float m = 0.0f, l = 0.0f;  // m: the maximum in use, in log2 units
+        bool ok = true;
+        for (uint32_t j = 0; j < n; ++j) {
+            ok = __all_sync(0xffffffffu, wait(&s_full[t], j & 1u));
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t s[128];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tmem_ld32(ts + 32u * i, s + 32 * i);
+            tmem_wait_ld();
+            const bool diagonal = j + 1 == n;
+            float hi = -INFINITY, lo = INFINITY;
+            if (diagonal) {
+#pragma unroll
+                for (int i = 0; i < 128; ++i) {
+                    if ((uint32_t)i <= r) {
+                        hi = fmaxf(hi, __uint_as_float(s[i]));
+                        lo = fminf(lo, __uint_as_float(s[i]));
+                    }
+                }
+            } else if (sc >= 0.0f) {
+                float h4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < 128; i += 8)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        h4[q] = fmaxf(fmaxf(h4[q], __uint_as_float(s[i + q])), __uint_as_float(s[i + q + 4]));
+                hi = fmaxf(fmaxf(h4[0], h4[1]), fmaxf(h4[2], h4[3]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 128; ++i) lo = fminf(lo, __uint_as_float(s[i]));
+            }
+            const float top = sc >= 0.0f ? hi * sc : lo * sc;
+            if (j == 0) {
+                m = top;
+            } else if (__any_sync(0xffffffffu, top > m + 8.0f)) {
+                const float mn = fmaxf(m, top);
+                const float f = mn == -INFINITY ? 1.0f : ex2_approx(m - mn);
+                l *= f;
+                m = mn;
+#pragma unroll 1
+                for (int i = 0; i < D; i += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(to + i, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                    tmem_st32(to + i, o);
+                }
+            }
+            const float base = 6.0f - (m == -INFINITY ? 0.0f : m);
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 128; i += 2) {
+                float a = ex2_approx(fmaf(__uint_as_float(s[i]), sc, base));
+                float b = ex2_approx(fmaf(__uint_as_float(s[i + 1]), sc, base));
+                if (diagonal) {
+                    a = (uint32_t)i <= r ? a : 0.0f;
+                    b = (uint32_t)(i + 1) <= r ? b : 0.0f;
+                }
+                sum[(i / 2) & 3] += a + b;
+                s[i / 2] = pack16<T>(a, b);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_st32(ts, s);
+            tmem_st32(ts + 32u, s + 32);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[t]);
+        }
+        if (n) {
+            if (ok) ok = __all_sync(0xffffffffu, wait(&o_full[t], 0));
+            if (ok) {
+                tc_fence_after();
+                const int64_t row = begin + row0 + t * 128 + r;
+                const bool mine = row0 + t * 128 + r < len;
+                const float inv = 1.0f / l;
+                bool fine = true;
+                const size_t at = (size_t)row * p.out_stride + (size_t)head * D;
+#pragma unroll 1
+                for (int i = 0; i < D; i += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(to + i, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 32; k += 8) {
+                        float x[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            x[e] = __uint_as_float(o[k + e]) * inv;
+                            fine = fine && fabsf(x[e]) < INFINITY;
+                        }
+                        if (mine) store8(p.out, p.out_type, at + i + k, x);
+                    }
+                }
+                uint32_t again = __ballot_sync(0xffffffffu, mine && !fine);
+                while (again) {
+                    const uint32_t k = __ffs(again) - 1u;
+                    again &= again - 1u;
+                    prompt_row<T, D>(p, begin, row - r + (warp & 3u) * 32u + k, head, lane);
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+    }
 }
 
 }  // namespace wl

@@ -91,13 +91,41 @@ int launch_kv_append(const KvAppendParams &p, dim3 grid, cudaStream_t s) {
     return WL_OK;
 }
 
+// Tensor map of [n_tokens][heads][D] 16-bit rows `stride` elements apart: 128 tokens
+// x 64 elements of one head, 128-byte swizzle, zeros behind the last token.
+int encode_heads(EncodeTiledFn enc, CUtensorMap *map, const void *base, uint32_t n_tokens,
+                 uint32_t heads, uint32_t D, uint64_t stride) {
+    const cuuint64_t dims[3] = {D, heads, n_tokens};
+    const cuuint64_t strides[2] = {D * 2ull, stride * 2ull};
+    const cuuint32_t box[3] = {64, 1, 128};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void *>(base), dims, strides, box,
+                     estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(WL_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return WL_OK;
+}
+
 template <typename T>
-int launch_attn_prompt(const AttnPromptParams &p, uint32_t head_dim, cudaStream_t s) {
-    const dim3 grid((p.n_tokens + 3u) / 4u, p.group * p.n_kv);
-    if (head_dim == 64)
-        WL_CUDA(launch(attn_prompt_rows_kernel<T, 64>, grid, dim3(128), 0, s, true, p));
+int launch_attn_prompt(const AttnPromptParams &p, uint32_t D, cudaStream_t s) {
+    EncodeTiledFn enc;
+    int rc = get_encode_tiled(&enc);
+    if (rc) return rc;
+    AttnPromptMaps maps;
+    if ((rc = encode_heads(enc, &maps.q, p.q, p.n_tokens, p.n_kv * p.group, D, p.q_stride)) ||
+        (rc = encode_heads(enc, &maps.k, p.k, p.n_tokens, p.n_kv, D, p.k_stride)) ||
+        (rc = encode_heads(enc, &maps.v, p.v, p.n_tokens, p.n_kv, D, p.v_stride)))
+        return rc;
+    // sequence s owns the units [seq_start[s] / 256 + s, ...), at least as many as it needs
+    const uint64_t ctas = ((uint64_t)p.n_tokens / PROMPT_ROWS + p.n_seqs) * p.n_kv * p.group;
+    if (ctas > 0x7FFFFFFFull)
+        return fail(WL_ERR_INVALID_ARGUMENT, "attn_prompt: %u tokens of %u sequences with %u heads",
+                    p.n_tokens, p.n_seqs, p.n_kv * p.group);
+    const dim3 grid((uint32_t)ctas), block(PROMPT_THREADS);
+    if (D == 64)
+        WL_CUDA(launch(attn_prompt_kernel<T, 64>, grid, block, PromptSmem<64>::DYN, s, true, maps, p));
     else
-        WL_CUDA(launch(attn_prompt_rows_kernel<T, 128>, grid, dim3(128), 0, s, true, p));
+        WL_CUDA(launch(attn_prompt_kernel<T, 128>, grid, block, PromptSmem<128>::DYN, s, true, maps, p));
     return WL_OK;
 }
 

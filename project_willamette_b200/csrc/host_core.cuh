@@ -170,7 +170,11 @@ int configure_kernels() {
                             (const void *)attn_gqa_batch_kernel<128, 1>,
                             (const void *)attn_gqa_batch_kernel<128, 2>,
                             (const void *)attn_gqa_batch_kernel<128, 3>,
-                            (const void *)attn_gqa_batch_kernel<128, 4>};
+                            (const void *)attn_gqa_batch_kernel<128, 4>,
+                            (const void *)attn_prompt_kernel<__half, 64>,
+                            (const void *)attn_prompt_kernel<__half, 128>,
+                            (const void *)attn_prompt_kernel<__nv_bfloat16, 64>,
+                            (const void *)attn_prompt_kernel<__nv_bfloat16, 128>};
     for (const void *k : others)
         WL_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      (int)kernel_dyn_cap(k)));
