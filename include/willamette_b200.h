@@ -406,7 +406,8 @@ int wl_dev_rope_kv_append_i8(const wl_kv_pages_i8 *cache, const wl_kv_append *ar
  * the cache: out = softmax(scale * q . k) v for each query head, zeros where
  * length[s] is 0.  Softmax and sums in f32.  workspace:
  * wl_attn_decode_workspace_bytes bytes, 16-byte aligned, zero before the first
- * call; every call leaves its counters zero again.  Calls that share a
+ * call; every call leaves its counters zero again (zero it anew after a call
+ * whose wait timed out, bit 0 of wl_device_status).  Calls that share a
  * workspace must not overlap on the GPU (graphs replayed side by side each
  * need their own). */
 typedef struct wl_attn_decode {

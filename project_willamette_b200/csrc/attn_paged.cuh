@@ -9,16 +9,18 @@
 // finite whatever they hold, and a page without a key below n is not read.
 #pragma once
 
+#include <cuda.h>
+
 #include <cstdint>
 
+#include "i2s_gemm.cuh"
 #include "kv_append.cuh"
 
 namespace wl {
 
 struct AttnDecodeParams {
-    const int8_t *kc, *vc;
     const float *ks, *vs;
-    uint32_t n_pages, page_size, n_kv, head_dim;
+    uint32_t n_pages, page_shift, n_kv;  // 2^page_shift keys a page
     const void *q;
     void *out;
     uint64_t q_stride, out_stride;
@@ -48,7 +50,7 @@ constexpr int PAGED_THREADS = 128;
 constexpr int PAGED_WARPS = PAGED_THREADS / 32;
 constexpr int PAGED_TILE = 32;                           // keys of a warp's step
 constexpr int PAGED_UNIT = PAGED_TILE * PAGED_WARPS;     // keys of a CTA's step: the unit of work
-constexpr int PAGED_CTAS_PER_SM = 3;
+constexpr int PAGED_CTAS_PER_SM = 2;
 constexpr int PAGED_MAX_CTAS = 148 * PAGED_CTAS_PER_SM;
 constexpr int PAGED_ROWS = 8;                            // query heads of one pass over the keys
 
@@ -66,21 +68,6 @@ __device__ __forceinline__ float ex2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
-}
-
-__device__ __forceinline__ uint4 ldg_stream16(const void *p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint2 ldg_stream8(const void *p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];"
-                 : "=r"(v.x), "=r"(v.y)
-                 : "l"(p));
-    return v;
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
@@ -108,32 +95,65 @@ __device__ __forceinline__ void split_f16(float v0, float v1, uint32_t &hi, uint
     lo = *reinterpret_cast<const uint32_t *>(&l);
 }
 
+template <int D>
+struct PagedSmem {
+    static constexpr uint32_t STAGES = D == 128 ? 3 : 6;
+    static constexpr uint32_t HALF = PAGED_TILE * D;   // a tile's keys; its values follow
+    static constexpr uint32_t STAGE = 2u * HALF;
+    static constexpr uint32_t WARP = STAGES * STAGE;
+    static constexpr size_t DYN = PAGED_WARPS * WARP + 1024;  // + alignment slack
+    static_assert(PAGED_ROWS * (D + 8) * 4 <= STAGE, "a warp's output rows fit a stage");
+};
+
+struct AttnDecodeMaps {
+    CUtensorMap k, v;  // all pages as rows of D bytes; box {D, min(32, page_size)}, swizzle of D bytes
+};
+
+// A contiguous run of one item's units, of one CTA.
+struct PagedSegment {
+    uint32_t seq, h, row0, rows;   // sequence, KV head, the pass's query heads within the group
+    uint32_t n, u0, u1, n_units;   // keys; units [u0, u1) of the item's n_units
+    uint64_t item0;                // the item's first unit
+};
+
 // One CTA of PAGED_CTAS_PER_SM per SM takes an equal, contiguous share of all
-// (sequence, KV head, pass, 128-key) units; its four warps take 32 keys each.
+// (sequence, KV head, pass, 128-key) units; its four warps take 32 keys each,
+// every warp through a ring of its own that it fills itself by TMA.
 template <int D>
 __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
-    attn_decode_i8_kernel(const AttnDecodeParams p) {
-    constexpr int KW = D / 64;   // 16-byte loads of a key row by one lane
+    attn_decode_i8_kernel(const __grid_constant__ AttnDecodeMaps maps, const AttnDecodeParams p) {
+    using L = PagedSmem<D>;
+    constexpr uint32_t ST = L::STAGES;
     constexpr int VW = D / 32;   // 4-byte words of a value row that one lane holds
     constexpr int NT = D / 8;    // output tiles of 8 dimensions
-    __shared__ float s_o[PAGED_WARPS][PAGED_ROWS][D + 8];
+    constexpr int OP = D + 8;    // pitch of an output row in shared memory
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t s_full[PAGED_WARPS][ST];
+    __shared__ int2 s_page[PAGED_WARPS][ST];   // a stage's page of each 16 keys, -1: none
     __shared__ float s_m[PAGED_WARPS][PAGED_ROWS], s_l[PAGED_WARPS][PAGED_ROWS];
     __shared__ unsigned long long s_scan[PAGED_WARPS];
     __shared__ unsigned long long s_start;
-    __shared__ uint32_t s_seq, s_last;
+    __shared__ uint32_t s_seq, s_last, s_abort;
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                                ~(uintptr_t)1023);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t g = lane >> 2, c = lane & 3u;  // the tile instructions' row and column group
-    const uint32_t P = p.page_size, passes = (p.group + PAGED_ROWS - 1) / PAGED_ROWS;
+    const uint32_t shift = p.page_shift, passes = (p.group + PAGED_ROWS - 1) / PAGED_ROWS;
     const uint32_t per = (p.group + passes - 1) / passes;  // query heads a pass
     const uint32_t items = p.n_kv * passes;                // items of a sequence
     const uint64_t b = blockIdx.x;
+    if (lane == 0)
+        for (uint32_t s = 0; s < ST; ++s) mbar_init(&s_full[warp][s], 1);
+    if (tid == 0) s_abort = 0;
+    fence_mbar_init();
     pdl_launch_dependents();
     pdl_wait();
 
     auto units_of = [&](uint32_t s) -> uint32_t {  // 0 for an empty or refused sequence
         const int64_t n = __ldg(p.length + s);
-        return n <= 0 || n > (int64_t)p.max_pages * P ? 0u
-                                                      : (uint32_t)((n + PAGED_UNIT - 1) / PAGED_UNIT);
+        return n <= 0 || n > ((int64_t)p.max_pages << shift)
+                   ? 0u
+                   : (uint32_t)((n + PAGED_UNIT - 1) / PAGED_UNIT);
     };
     // rows of sequences without keys
     for (uint32_t s = (uint32_t)b; s < p.n_seqs; s += gridDim.x) {
@@ -186,27 +206,121 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
         }
         __syncthreads();
     }
-    uint32_t seq = s_seq;
-    uint64_t seq_unit = s_start;  // the sequence's first unit
-    uint64_t at = begin;
-    uint32_t n_units = units_of(seq);
     auto *counters = static_cast<uint32_t *>(p.workspace);
     auto *ml = reinterpret_cast<float2 *>(static_cast<uint8_t *>(p.workspace) + paged_ml_offset());
     auto *po = reinterpret_cast<float *>(static_cast<uint8_t *>(p.workspace) + paged_o_offset());
 
-    while (at < end) {
-        while (at >= seq_unit + (uint64_t)n_units * items) {  // the next sequence with keys
-            seq_unit += (uint64_t)n_units * items;
+    uint32_t seq = s_seq;
+    uint64_t seq_unit = s_start;  // the sequence's first unit
+    auto segment_at = [&](uint64_t at) {  // at < end, ascending from call to call
+        uint32_t nu = units_of(seq);
+        while (at >= seq_unit + (uint64_t)nu * items) {  // the next sequence with keys
+            seq_unit += (uint64_t)nu * items;
             ++seq;
-            n_units = units_of(seq);
+            nu = units_of(seq);
         }
-        const uint32_t item = (uint32_t)((at - seq_unit) / n_units);
-        const uint64_t item0 = seq_unit + (uint64_t)item * n_units, item1 = item0 + n_units;
-        const uint32_t u0 = (uint32_t)(at - item0), u1 = (uint32_t)(min(end, item1) - item0);
-        const uint32_t h = item / passes, pass = item % passes;
-        const uint32_t n = (uint32_t)__ldg(p.length + seq);
-        const uint32_t row0 = pass * per, rows = min(per, p.group - row0);
-        const uint32_t head = h * p.group + row0;
+        PagedSegment s;
+        const uint32_t item = (uint32_t)((at - seq_unit) / nu), pass = item % passes;
+        s.seq = seq;
+        s.h = item / passes;
+        s.row0 = pass * per;
+        s.rows = min(per, p.group - s.row0);
+        s.n = (uint32_t)__ldg(p.length + seq);
+        s.n_units = nu;
+        s.item0 = seq_unit + (uint64_t)item * nu;
+        s.u0 = (uint32_t)(at - s.item0);
+        s.u1 = (uint32_t)(min(end, s.item0 + nu) - s.item0);
+        return s;
+    };
+    auto page_at = [&](const PagedSegment &s, uint32_t t) -> int32_t {  // of key t < n, -1 if refused
+        const int32_t page = __ldg(p.page_table + (size_t)s.seq * p.max_pages + (t >> shift));
+        if (page >= 0 && (uint32_t)page < p.n_pages) return page;
+        atomicOr(p.status, WL_DEV_ERR_INDEX);
+        return -1;
+    };
+    // pages of this warp's tile of unit u: keys [u * UNIT + warp * TILE, + TILE)
+    auto pages_of = [&](const PagedSegment &s, uint32_t u) {
+        const uint32_t t = u * PAGED_UNIT + warp * PAGED_TILE;
+        int2 r = make_int2(-1, -1);
+        if (t < s.n) r.x = r.y = page_at(s, t);
+        if (shift == 4u) r.y = t + 16u < s.n ? page_at(s, t + 16u) : -1;
+        return r;
+    };
+    uint8_t *ring = smem + warp * L::WARP;
+    uint32_t issued = 0;  // (lane 0) ring entries filled
+    // (lane 0) the tile of unit u into ring entry `entry`, each in turn
+    auto issue = [&](const PagedSegment &s, uint32_t u, uint32_t entry, int2 page) {
+        issued = entry + 1u;
+        const uint32_t st = entry % ST, t = u * PAGED_UNIT + warp * PAGED_TILE;
+        uint8_t *dst = ring + st * L::STAGE;
+        uint64_t *bar = &s_full[warp][st];
+        s_page[warp][st] = page;
+        if (shift != 4u) {
+            mbar_arrive_expect_tx(bar, page.x >= 0 ? L::STAGE : 0u);
+            if (page.x >= 0) {
+                const uint32_t row = (((uint32_t)page.x * p.n_kv + s.h) << shift) + (t & ((1u << shift) - 1u));
+                tma_load_2d_plain(dst, &maps.k, 0, row, bar);
+                tma_load_2d_plain(dst + L::HALF, &maps.v, 0, row, bar);
+            }
+        } else {
+            mbar_arrive_expect_tx(bar, ((page.x >= 0) + (page.y >= 0)) * (L::STAGE / 2u));
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                const int32_t pg = a ? page.y : page.x;
+                if (pg >= 0) {
+                    const uint32_t row = ((uint32_t)pg * p.n_kv + s.h) << 4;
+                    tma_load_2d_plain(dst + a * (L::HALF / 2u), &maps.k, 0, row, bar);
+                    tma_load_2d_plain(dst + L::HALF + a * (L::HALF / 2u), &maps.v, 0, row, bar);
+                }
+            }
+        }
+    };
+    // lane's places in a stage: keys' row g, 16-byte pieces of its four dimensions
+    // groups; values' rows 2c, 2c + 1 (and 8 more, 16 more), its D / 8 dimensions
+    uint32_t koff[D / 64], voff[2];
+    if constexpr (D == 128) {
+        koff[0] = g * 128u + (((2u * c) ^ g) << 4);
+        koff[1] = g * 128u + (((2u * c + 1u) ^ g) << 4);
+        voff[0] = 2u * c * 128u + ((g ^ (2u * c)) << 4);
+        voff[1] = (2u * c + 1u) * 128u + ((g ^ (2u * c + 1u)) << 4);
+    } else {
+        koff[0] = g * 64u + ((c ^ ((g >> 1) & 3u)) << 4);
+        voff[0] = 2u * c * 64u + (((g >> 1) ^ c) << 4) + (g & 1u) * 8u;
+        voff[1] = voff[0] + 64u;
+    }
+
+    uint64_t at = begin;
+    uint32_t it = 0;                     // ring entries consumed
+    PagedSegment sg = segment_at(at);
+    if (lane == 0)
+        for (uint32_t i = 0; i < ST - 1u && sg.u0 + i < sg.u1; ++i)
+            issue(sg, sg.u0 + i, it + i, pages_of(sg, sg.u0 + i));
+    bool ok = true;
+    for (;;) {
+        const uint32_t head = sg.h * p.group + sg.row0;
+        // the entry that the joining of the segment before had used, and the pages
+        // of the one after it
+        int2 ahead = make_int2(-1, -1);
+        if (lane == 0) {
+            if (sg.u0 + ST - 1u < sg.u1) issue(sg, sg.u0 + ST - 1u, it + ST - 1u, pages_of(sg, sg.u0 + ST - 1u));
+            if (sg.u0 + ST < sg.u1) ahead = pages_of(sg, sg.u0 + ST);
+        }
+        __syncwarp();
+        const float *ksh = p.ks + sg.h, *vsh = p.vs + sg.h;
+        auto scales = [&](uint32_t entry, int2 &page, float (&s)[4]) {
+            page = s_page[warp][entry % ST];
+            s[0] = page.x >= 0 ? __ldg(ksh + (size_t)page.x * p.n_kv) : 0.0f;
+            s[1] = page.x >= 0 ? __ldg(vsh + (size_t)page.x * p.n_kv) : 0.0f;
+            s[2] = s[0];
+            s[3] = s[1];
+            if (shift == 4u) {
+                s[2] = page.y >= 0 ? __ldg(ksh + (size_t)page.y * p.n_kv) : 0.0f;
+                s[3] = page.y >= 0 ? __ldg(vsh + (size_t)page.y * p.n_kv) : 0.0f;
+            }
+        };
+        int2 page;
+        float sc[4];
+        scales(it, page, sc);
 
         // the pass's query rows: row g as f16 parts hi (tile row g) and lo (row
         // g + 8) of q * 2^shift, its largest |q| brought to [2^13, 2^14)
@@ -217,12 +331,12 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
             float top = 0.0f;
 #pragma unroll
             for (int j = 0; j < D / 16; ++j) {
-                const uint32_t d = (j < 4 ? c * 16u + 4u * j : 64u + c * 16u + 4u * (j - 4));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    x[4 * j + i] = g < rows ? load_typed(p.q, p.type, seq * p.q_stride +
-                                                                          (size_t)(head + g) * D + d + i)
-                                            : 0.0f;
+                    x[4 * j + i] =
+                        g < sg.rows ? load_typed(p.q, p.type, sg.seq * p.q_stride + (size_t)(head + g) * D +
+                                                                  c * (D / 4) + 4 * j + i)
+                                    : 0.0f;
                     top = fmaxf(top, fabsf(x[4 * j + i]));
                 }
             }
@@ -245,238 +359,227 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
 #pragma unroll
         for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 
-        // keys of this warp's tile of unit u: [u * UNIT + warp * TILE, + TILE), in two
-        // halves of 16 that each lie in one page
-        uint4 kr[4][KW];
-        int32_t pid[2];
-        float ks[2], vs[2];
-        auto fetch_page = [&](uint32_t u) {
+        for (uint32_t u = sg.u0; u < sg.u1; ++u, ++it) {
             const uint32_t t0 = u * PAGED_UNIT + warp * PAGED_TILE;
+            const uint8_t *st = ring + (it % ST) * L::STAGE;
+            int2 page_next = make_int2(-1, -1);
+            float sc_next[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (u + 1 < sg.u1) scales(it + 1, page_next, sc_next);
+            ok = __all_sync(0xffffffffu, mbar_wait(&s_full[warp][it % ST], (it / ST) & 1u));
+            if (!ok) break;
+            if (page.x >= 0 || page.y >= 0) {
+                float s[4][4];
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                const uint32_t t = t0 + 16u * a;
-                pid[a] = t < n ? __ldg(p.page_table + (size_t)seq * p.max_pages + t / P) : -1;
-                if (t < n && (pid[a] < 0 || (uint32_t)pid[a] >= p.n_pages)) {
-                    if (lane == 0) atomicOr(p.status, WL_DEV_ERR_INDEX);
-                    pid[a] = -1;
+                for (int t = 0; t < 4; ++t) {
+                    s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < D / 64; ++w) {
+                        const uint4 r = lds128(st + koff[w] + t * 8 * D);
+                        const uint32_t x[4] = {r.x ^ 0x80808080u, r.y ^ 0x80808080u, r.z ^ 0x80808080u,
+                                               r.w ^ 0x80808080u};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            mma_f16(s[t], qa[4 * w + j], unbias(__byte_perm(x[j], EXP1024, 0x4140)),
+                                    unbias(__byte_perm(x[j], EXP1024, 0x4342)));
+                    }
                 }
-            }
-        };
-        auto block_of = [&](int32_t page) { return (size_t)page * p.n_kv + h; };
-        auto load_k = [&](uint32_t u) {
-            const uint32_t t0 = u * PAGED_UNIT + warp * PAGED_TILE;
+                // z in log2 units, keys 2c, 2c+1 of each 8
+                float z[4][2];
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                if (pid[a] >= 0) {
-                    const size_t block = block_of(pid[a]);
-                    ks[a] = __ldg(p.ks + block);
-                    vs[a] = __ldg(p.vs + block);
-                    const int8_t *k = p.kc + (block * P + ((t0 + 16u * a) & (P - 1u)) + g) * D + c * 16u;
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int w = 0; w < KW; ++w)
-                            kr[2 * a + i][w] = ldg_stream16(k + 8 * i * D + 64 * w);
-                } else {
-                    ks[a] = vs[a] = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int w = 0; w < KW; ++w) kr[2 * a + i][w] = make_uint4(0, 0, 0, 0);
+                for (int t = 0; t < 4; ++t) {
+                    const float f = qf * sc[t < 2 ? 0 : 2];
+                    z[t][0] = (s[t][0] + s[t][2]) * f;
+                    z[t][1] = (s[t][1] + s[t][3]) * f;
                 }
-            }
-        };
-        fetch_page(u0);
-        load_k(u0);
-        for (uint32_t u = u0; u < u1; ++u) {
-            const uint32_t t0 = u * PAGED_UNIT + warp * PAGED_TILE;
-            // this step's values, used after the softmax
-            uint32_t vr[2][4][VW];
-            const float ks0 = ks[0], ks1 = ks[1], vs0 = vs[0], vs1 = vs[1];
-            const bool here[2] = {pid[0] >= 0, pid[1] >= 0};
+                if (t0 + PAGED_TILE > sg.n || page.x < 0 || page.y < 0) {  // keys that take no part
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                const int8_t *v = p.vc + (block_of(max(pid[a], 0)) * P + ((t0 + 16u * a) & (P - 1u))) * D +
-                                  g * (D / 8);
+                    for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint32_t t = 2u * c + (r & 1) + 8u * (r >> 1);
-                    if (here[a]) {
+                        for (int i = 0; i < 2; ++i)
+                            if (t0 + 8u * t + 2u * c + i >= sg.n || (t < 2 ? page.x : page.y) < 0)
+                                z[t][i] = -INFINITY;
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int t = 0; t < 4; ++t) top = fmaxf(top, fmaxf(z[t][0], z[t][1]));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float vtop = fmaxf(fabsf(sc[1]), fabsf(sc[3]));
+                if (__any_sync(0xffffffffu, top > m) || vtop > vref) {
+                    const float mn = fmaxf(m, top), vn = fmaxf(vref, vtop);
+                    const float shrink = mn == -INFINITY ? 0.0f : ex2_approx(m - mn);
+                    const float f = vn > 0.0f ? shrink * (vref / vn) : 0.0f;
+                    l *= shrink;
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) {
+                        o[i][0] *= f;
+                        o[i][1] *= f;
+                        o[i][2] *= f;
+                        o[i][3] *= f;
+                    }
+                    m = mn;
+                    vref = vn;
+                }
+                // weights times 2^14, so that the f16 parts of small ones keep their bits,
+                // and relative to the largest scale of the values so far
+                const float base = 14.0f - (m == -INFINITY ? 0.0f : m);
+                const float r0 = sc[1] == 0.0f ? 0.0f : sc[1] / vref, r1 = sc[3] == 0.0f ? 0.0f : sc[3] / vref;
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    uint32_t w[4];
+                    const float r = a ? r1 : r0;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float e0 = ex2_approx(z[2 * a + i][0] + base);
+                        const float e1 = ex2_approx(z[2 * a + i][1] + base);
+                        l += e0 + e1;
+                        split_f16(e0 * r, e1 * r, w[2 * i], w[2 * i + 1]);
+                    }
+                    uint32_t v[4][VW];  // value rows 2c, 2c + 1, 2c + 8, 2c + 9 of these 16 keys
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint8_t *src = st + L::HALF + voff[k & 1] + (16 * a + 8 * (k >> 1)) * D;
                         if constexpr (D == 128) {
-                            const uint4 w = ldg_stream16(v + t * D);
-                            vr[a][r][0] = w.x;
-                            vr[a][r][1] = w.y;
-                            vr[a][r][2] = w.z;
-                            vr[a][r][3] = w.w;
+                            const uint4 y = lds128(src);
+                            v[k][0] = y.x ^ 0x80808080u;
+                            v[k][1] = y.y ^ 0x80808080u;
+                            v[k][2] = y.z ^ 0x80808080u;
+                            v[k][3] = y.w ^ 0x80808080u;
                         } else {
-                            const uint2 w = ldg_stream8(v + t * D);
-                            vr[a][r][0] = w.x;
-                            vr[a][r][1] = w.y;
+                            const uint2 y = *reinterpret_cast<const uint2 *>(src);
+                            v[k][0] = y.x ^ 0x80808080u;
+                            v[k][1] = y.y ^ 0x80808080u;
                         }
-                    } else {
+                    }
 #pragma unroll
-                        for (int w = 0; w < VW; ++w) vr[a][r][w] = 0u;
+                    for (int i = 0; i < VW; ++i) {
+                        const uint32_t a01 = __byte_perm(v[0][i], v[1][i], 0x5140);
+                        const uint32_t a23 = __byte_perm(v[0][i], v[1][i], 0x7362);
+                        const uint32_t b01 = __byte_perm(v[2][i], v[3][i], 0x5140);
+                        const uint32_t b23 = __byte_perm(v[2][i], v[3][i], 0x7362);
+                        mma_f16(o[4 * i], w, unbias(__byte_perm(a01, EXP1024, 0x4140)),
+                                unbias(__byte_perm(b01, EXP1024, 0x4140)));
+                        mma_f16(o[4 * i + 1], w, unbias(__byte_perm(a01, EXP1024, 0x4342)),
+                                unbias(__byte_perm(b01, EXP1024, 0x4342)));
+                        mma_f16(o[4 * i + 2], w, unbias(__byte_perm(a23, EXP1024, 0x4140)),
+                                unbias(__byte_perm(b23, EXP1024, 0x4140)));
+                        mma_f16(o[4 * i + 3], w, unbias(__byte_perm(a23, EXP1024, 0x4342)),
+                                unbias(__byte_perm(b23, EXP1024, 0x4342)));
                     }
                 }
             }
-            if (u + 1 < u1) fetch_page(u + 1);
-
-            float s[4][4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
-#pragma unroll
-                for (int j = 0; j < D / 16; ++j) {
-                    const uint4 &r = kr[t][j / 4];
-                    const uint32_t x =
-                        (j % 4 == 0 ? r.x : j % 4 == 1 ? r.y : j % 4 == 2 ? r.z : r.w) ^ 0x80808080u;
-                    mma_f16(s[t], qa[j], unbias(__byte_perm(x, EXP1024, 0x4140)),
-                            unbias(__byte_perm(x, EXP1024, 0x4342)));
-                }
+            __syncwarp();  // the entry is free again
+            if (lane == 0 && u + ST < sg.u1) {
+                issue(sg, u + ST, it + ST, ahead);
+                if (u + ST + 1u < sg.u1) ahead = pages_of(sg, u + ST + 1u);
             }
-            if (u + 1 < u1) load_k(u + 1);
-
-            // z in log2 units, keys 2c, 2c+1 of each 8; masked at the length and where
-            // the page was refused
-            float z[4][2];
-            float top = -INFINITY;
+            __syncwarp();
+            page = page_next;
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const float f = qf * (t < 2 ? ks0 : ks1);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t key = t0 + 8u * t + 2u * c + i;
-                    z[t][i] = key < n && here[t / 2] ? (s[t][i] + s[t][i + 2]) * f : -INFINITY;
-                    top = fmaxf(top, z[t][i]);
-                }
+            for (int i = 0; i < 4; ++i) sc[i] = sc_next[i];
+        }
+        if (!ok) {
+            if (lane == 0) {
+                atomicOr(p.status - 1, WL_DEV_ERR_TIMEOUT);
+                *(volatile uint32_t *)&s_abort = 1u;
             }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float vtop = fmaxf(fabsf(vs0), fabsf(vs1));
-            if (__any_sync(0xffffffffu, top > m) || vtop > vref) {
-                const float mn = fmaxf(m, top), vn = fmaxf(vref, vtop);
-                const float shrink = mn == -INFINITY ? 0.0f : ex2_approx(m - mn);
-                const float f = vn > 0.0f ? shrink * (vref / vn) : 0.0f;
-                l *= shrink;
-#pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    o[i][0] *= f;
-                    o[i][1] *= f;
-                    o[i][2] *= f;
-                    o[i][3] *= f;
-                }
-                m = mn;
-                vref = vn;
-            }
-            // weights times 2^14, so that the f16 parts of small ones keep their bits
-            const float base = 14.0f - (m == -INFINITY ? 0.0f : m);
-            const float r0 = vs0 == 0.0f ? 0.0f : vs0 / vref, r1 = vs1 == 0.0f ? 0.0f : vs1 / vref;
-#pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                uint32_t w[4];
-                const float r = a ? r1 : r0;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float e0 = ex2_approx(z[2 * a + i][0] + base);
-                    const float e1 = ex2_approx(z[2 * a + i][1] + base);
-                    l += e0 + e1;
-                    split_f16(e0 * r, e1 * r, w[2 * i], w[2 * i + 1]);
-                }
-#pragma unroll
-                for (int i = 0; i < VW; ++i) {
-                    uint32_t x[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) x[k] = vr[a][k][i] ^ 0x80808080u;
-                    const uint32_t a01 = __byte_perm(x[0], x[1], 0x5140), a23 = __byte_perm(x[0], x[1], 0x7362);
-                    const uint32_t b01 = __byte_perm(x[2], x[3], 0x5140), b23 = __byte_perm(x[2], x[3], 0x7362);
-                    mma_f16(o[4 * i], w, unbias(__byte_perm(a01, EXP1024, 0x4140)),
-                            unbias(__byte_perm(b01, EXP1024, 0x4140)));
-                    mma_f16(o[4 * i + 1], w, unbias(__byte_perm(a01, EXP1024, 0x4342)),
-                            unbias(__byte_perm(b01, EXP1024, 0x4342)));
-                    mma_f16(o[4 * i + 2], w, unbias(__byte_perm(a23, EXP1024, 0x4140)),
-                            unbias(__byte_perm(b23, EXP1024, 0x4140)));
-                    mma_f16(o[4 * i + 3], w, unbias(__byte_perm(a23, EXP1024, 0x4342)),
-                            unbias(__byte_perm(b23, EXP1024, 0x4342)));
-                }
-            }
+        }
+        // the next segment's first tiles into the entries that the joining does not use
+        at = sg.item0 + sg.u1;
+        const PagedSegment done = sg;
+        if (at < end) {
+            sg = segment_at(at);
+            if (ok && lane == 0)
+                for (uint32_t i = 0; i < ST - 1u && sg.u0 + i < sg.u1; ++i)
+                    issue(sg, sg.u0 + i, it + i, pages_of(sg, sg.u0 + i));
         }
         // the warps' shares of the segment, joined in warp order.  Output tile i,
         // column n stands for dimension n * D / 8 + i; kept at 8 i + n.
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         const float back = vref * 6.103515625e-05f;  // 2^-14
+        const uint32_t free_at = ((it + ST - 1u) % ST) * L::STAGE;  // the same in every warp
+        float *so = reinterpret_cast<float *>(ring + free_at);
 #pragma unroll
         for (int i = 0; i < NT; ++i)
-            *reinterpret_cast<float2 *>(&s_o[warp][g][8 * i + 2 * c]) =
+            *reinterpret_cast<float2 *>(so + g * OP + 8 * i + 2 * c) =
                 make_float2((o[i][0] + o[i][2]) * back, (o[i][1] + o[i][3]) * back);
         if (c == 0) {
             s_m[warp][g] = m;
             s_l[warp][g] = l * 6.103515625e-05f;
         }
         __syncthreads();
-        const bool whole = u0 == 0 && u1 == n_units;
-        const bool tail = u0 != 0;
-        const size_t slot = (size_t)b * 2u + (tail ? 0u : 1u);
-        for (uint32_t i = tid; i < rows * D; i += PAGED_THREADS) {
-            const uint32_t r = i / D, k = i % D;
-            float mx = -INFINITY;
+        const bool stop = s_abort != 0u;  // a wait ran out: nothing more is read or written
+        const bool whole = done.u0 == 0 && done.u1 == done.n_units;
+        const size_t slot = (size_t)b * 2u + (done.u0 != 0 ? 0u : 1u);
+        if (!stop) {
+            for (uint32_t i = tid; i < done.rows * D; i += PAGED_THREADS) {
+                const uint32_t r = i / D, k = i % D;
+                float mx = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < PAGED_WARPS; ++w) mx = fmaxf(mx, s_m[w][r]);
-            const float ref = mx == -INFINITY ? 0.0f : mx;
-            float sum = 0.0f, acc = 0.0f;
+                for (int w = 0; w < PAGED_WARPS; ++w) mx = fmaxf(mx, s_m[w][r]);
+                const float ref = mx == -INFINITY ? 0.0f : mx;
+                float sum = 0.0f, acc = 0.0f;
 #pragma unroll
-            for (int w = 0; w < PAGED_WARPS; ++w) {
-                const float f = ex2_approx(s_m[w][r] - ref);
-                sum = fmaf(s_l[w][r], f, sum);
-                acc = fmaf(s_o[w][r][k], f, acc);
-            }
-            if (whole) {
-                const uint32_t d = (k & 7u) * (D / 8) + (k >> 3);
-                store_typed(p.out, p.out_type, seq * p.out_stride + (size_t)(head + r) * D + d,
-                            sum == 0.0f ? 0.0f : acc / sum);
-            } else {
-                po[(slot * PAGED_ROWS + r) * D + k] = acc;
-                if (k == 0) ml[slot * PAGED_ROWS + r] = make_float2(mx, sum);
-            }
-        }
-        if (!whole) {
-            // the CTAs that share the item: the last to arrive joins their parts in order
-            const uint32_t first = (uint32_t)(((item0 + 1) * N - 1) / total);
-            const uint32_t last = (uint32_t)((item1 * N - 1) / total);
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) {
-                const uint32_t before = atomicAdd(counters + first, 1u);
-                s_last = before == last - first;
-                if (s_last) counters[first] = 0u;
-                __threadfence();
-            }
-            __syncthreads();
-            if (s_last) {
-                for (uint32_t i = tid; i < rows * D; i += PAGED_THREADS) {
-                    const uint32_t r = i / D, k = i % D;
-                    float mx = -INFINITY;
-                    for (uint32_t x = first; x <= last; ++x)
-                        mx = fmaxf(mx, __ldcg(&ml[((size_t)x * 2u + (x == first)) * PAGED_ROWS + r]).x);
-                    const float ref = mx == -INFINITY ? 0.0f : mx;
-                    float sum = 0.0f, acc = 0.0f;
-#pragma unroll 4
-                    for (uint32_t x = first; x <= last; ++x) {
-                        const size_t y = ((size_t)x * 2u + (x == first)) * PAGED_ROWS + r;
-                        const float2 v = __ldcg(&ml[y]);
-                        const float f = ex2_approx(v.x - ref);
-                        sum = fmaf(v.y, f, sum);
-                        acc = fmaf(__ldcg(&po[y * D + k]), f, acc);
-                    }
+                for (int w = 0; w < PAGED_WARPS; ++w) {
+                    const float f = ex2_approx(s_m[w][r] - ref);
+                    sum = fmaf(s_l[w][r], f, sum);
+                    acc = fmaf(reinterpret_cast<const float *>(smem + w * L::WARP + free_at)[r * OP + k], f, acc);
+                }
+                if (whole) {
                     const uint32_t d = (k & 7u) * (D / 8) + (k >> 3);
-                    store_typed(p.out, p.out_type, seq * p.out_stride + (size_t)(head + r) * D + d,
+                    store_typed(p.out, p.out_type, done.seq * p.out_stride + (size_t)(head + r) * D + d,
                                 sum == 0.0f ? 0.0f : acc / sum);
+                } else {
+                    po[(slot * PAGED_ROWS + r) * D + k] = acc;
+                    if (k == 0) ml[slot * PAGED_ROWS + r] = make_float2(mx, sum);
+                }
+            }
+            if (!whole) {
+                // the CTAs that share the item: the last to arrive joins their parts in order
+                const uint32_t first = (uint32_t)(((done.item0 + 1) * N - 1) / total);
+                const uint32_t last = (uint32_t)(((done.item0 + done.n_units) * N - 1) / total);
+                __threadfence();
+                __syncthreads();
+                if (tid == 0) {
+                    const uint32_t before = atomicAdd(counters + first, 1u);
+                    s_last = before == last - first;
+                    if (s_last) counters[first] = 0u;
+                    __threadfence();
+                }
+                __syncthreads();
+                if (s_last) {
+                    for (uint32_t i = tid; i < done.rows * D; i += PAGED_THREADS) {
+                        const uint32_t r = i / D, k = i % D;
+                        float mx = -INFINITY;
+                        for (uint32_t x = first; x <= last; ++x)
+                            mx = fmaxf(mx, __ldcg(&ml[((size_t)x * 2u + (x == first)) * PAGED_ROWS + r]).x);
+                        const float ref = mx == -INFINITY ? 0.0f : mx;
+                        float sum = 0.0f, acc = 0.0f;
+#pragma unroll 4
+                        for (uint32_t x = first; x <= last; ++x) {
+                            const size_t y = ((size_t)x * 2u + (x == first)) * PAGED_ROWS + r;
+                            const float2 v = __ldcg(&ml[y]);
+                            const float f = ex2_approx(v.x - ref);
+                            sum = fmaf(v.y, f, sum);
+                            acc = fmaf(__ldcg(&po[y * D + k]), f, acc);
+                        }
+                        const uint32_t d = (k & 7u) * (D / 8) + (k >> 3);
+                        store_typed(p.out, p.out_type, done.seq * p.out_stride + (size_t)(head + r) * D + d,
+                                    sum == 0.0f ? 0.0f : acc / sum);
+                    }
                 }
             }
         }
-        __syncthreads();  // s_o is free again
-        at = item0 + u1;
+        if (at >= end || stop) break;
+        // the joining's reads and writes of the ring come before the copy that follows
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
     }
+    // after a wait that ran out: (bounded) the copies still in flight land before
+    // the CTA's shared memory goes
+    if (lane == 0)
+        for (; it < issued; ++it) (void)mbar_wait(&s_full[warp][it % ST], (it / ST) & 1u);
 }
 
 }  // namespace wl

@@ -12,7 +12,6 @@
 #include <cstdint>
 
 #include "attn_paged.cuh"
-#include "i2s_gemm.cuh"
 
 namespace wl {
 

@@ -55,9 +55,19 @@ int check_kv_pages(const char *op, const wl_kv_pages_i8 *c) {
     if (!c->k_scale || !c->v_scale || (reinterpret_cast<uintptr_t>(c->k_scale) & 3u) ||
         (reinterpret_cast<uintptr_t>(c->v_scale) & 3u))
         return fail(WL_ERR_INVALID_ARGUMENT, "%s: page scales NULL or not 4-byte aligned", op);
-    if (!c->n_pages || c->n_pages > 0x7FFFFFFFu)
-        return fail(WL_ERR_INVALID_ARGUMENT, "%s: %u pages", op, c->n_pages);
+    if (!c->n_pages || (uint64_t)c->n_pages * c->n_kv_heads * c->page_size > 0x7FFFFFFFull)
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: %u pages of %u heads (at most 2^31 - 1 rows)", op,
+                    c->n_pages, c->n_kv_heads);
     return WL_OK;
+}
+
+// Tensor map of a cache's codes as rows of head_dim bytes: up to 32 rows of one page
+// and head a copy, the swizzle that spans a row.
+int encode_pages(EncodeTiledFn enc, CUtensorMap *map, const int8_t *codes, const wl_kv_pages_i8 *c) {
+    const uint32_t D = c->head_dim;
+    const uint64_t rows = (uint64_t)c->n_pages * c->n_kv_heads * c->page_size;
+    return encode_2d(enc, map, codes, D, rows, D, std::min(c->page_size, 32u),
+                     D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 // Where these operators report a bad index read on the device: the second
@@ -252,14 +262,16 @@ int wl_dev_attn_decode_i8(const wl_kv_pages_i8 *cache, const wl_attn_decode *a, 
     AttnDecodeParams p;
     memset(&p, 0, sizeof p);
     if ((rc = attn_status(op, &p.status))) return rc;
-    p.kc = cache->k;
-    p.vc = cache->v;
+    EncodeTiledFn enc;
+    AttnDecodeMaps maps;
+    if ((rc = get_encode_tiled(&enc)) || (rc = encode_pages(enc, &maps.k, cache->k, cache)) ||
+        (rc = encode_pages(enc, &maps.v, cache->v, cache)))
+        return rc;
     p.ks = cache->k_scale;
     p.vs = cache->v_scale;
     p.n_pages = cache->n_pages;
-    p.page_size = cache->page_size;
+    p.page_shift = (uint32_t)__builtin_ctz(cache->page_size);
     p.n_kv = KV;
-    p.head_dim = D;
     p.q = a->q;
     p.out = a->out;
     p.q_stride = a->q_stride;
@@ -276,11 +288,11 @@ int wl_dev_attn_decode_i8(const wl_kv_pages_i8 *cache, const wl_attn_decode *a, 
     const uint32_t ctas = std::min<uint32_t>((uint32_t)sm_count_for_launch() * PAGED_CTAS_PER_SM,
                                              PAGED_MAX_CTAS);
     if (D == 64)
-        WL_CUDA(launch(attn_decode_i8_kernel<64>, dim3(ctas), dim3(PAGED_THREADS), 0,
-                       (cudaStream_t)stream, true, p));
+        WL_CUDA(launch(attn_decode_i8_kernel<64>, dim3(ctas), dim3(PAGED_THREADS), PagedSmem<64>::DYN,
+                       (cudaStream_t)stream, true, maps, p));
     else
-        WL_CUDA(launch(attn_decode_i8_kernel<128>, dim3(ctas), dim3(PAGED_THREADS), 0,
-                       (cudaStream_t)stream, true, p));
+        WL_CUDA(launch(attn_decode_i8_kernel<128>, dim3(ctas), dim3(PAGED_THREADS), PagedSmem<128>::DYN,
+                       (cudaStream_t)stream, true, maps, p));
     return WL_OK;
 }
 

@@ -171,6 +171,8 @@ int configure_kernels() {
                             (const void *)attn_gqa_batch_kernel<128, 2>,
                             (const void *)attn_gqa_batch_kernel<128, 3>,
                             (const void *)attn_gqa_batch_kernel<128, 4>,
+                            (const void *)attn_decode_i8_kernel<64>,
+                            (const void *)attn_decode_i8_kernel<128>,
                             (const void *)attn_prompt_kernel<__half, 64>,
                             (const void *)attn_prompt_kernel<__half, 128>,
                             (const void *)attn_prompt_kernel<__nv_bfloat16, 64>,
