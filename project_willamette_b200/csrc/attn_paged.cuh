@@ -116,20 +116,60 @@ struct PagedSegment {
     uint64_t item0;                // the item's first unit
 };
 
+__device__ __forceinline__ uint64_t div_fast(uint64_t a, uint32_t b) {
+    return a >> 32 ? a / b : (uint64_t)((uint32_t)a / b);
+}
+
+// W = D / 4 consecutive elements as f32.
+template <int W>
+__device__ __forceinline__ void load_row_part(const void *base, uint32_t type, size_t at, float (&x)[W]) {
+    if (type == 0u) {
+        const float4 *src = reinterpret_cast<const float4 *>(static_cast<const float *>(base) + at);
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i) {
+            const float4 v = __ldg(src + i);
+            x[4 * i] = v.x;
+            x[4 * i + 1] = v.y;
+            x[4 * i + 2] = v.z;
+            x[4 * i + 3] = v.w;
+        }
+        return;
+    }
+    const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + at);
+    uint4 raw[W / 8];
+#pragma unroll
+    for (int i = 0; i < W / 8; ++i) raw[i] = __ldg(src + i);
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) {
+        const uint32_t u = i % 4 == 0 ? raw[i / 4].x : i % 4 == 1 ? raw[i / 4].y : i % 4 == 2 ? raw[i / 4].z : raw[i / 4].w;
+        if (type == 1u) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u));
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        } else {
+            x[2 * i] = __uint_as_float(u << 16);
+            x[2 * i + 1] = __uint_as_float(u & 0xFFFF0000u);
+        }
+    }
+}
+
 // One CTA of PAGED_CTAS_PER_SM per SM takes an equal, contiguous share of all
 // (sequence, KV head, pass, 128-key) units; its four warps take 32 keys each,
 // every warp through a ring of its own that it fills itself by TMA.
-template <int D>
+// SMALL: pages of 16 keys, two to a tile; else a tile lies in one page.
+template <int D, bool SMALL>
 __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
     attn_decode_i8_kernel(const __grid_constant__ AttnDecodeMaps maps, const AttnDecodeParams p) {
     using L = PagedSmem<D>;
     constexpr uint32_t ST = L::STAGES;
+    constexpr int KW = D / 64;   // 16-byte pieces of a key row that one lane holds
     constexpr int VW = D / 32;   // 4-byte words of a value row that one lane holds
     constexpr int NT = D / 8;    // output tiles of 8 dimensions
     constexpr int OP = D + 8;    // pitch of an output row in shared memory
+    constexpr int HN = SMALL ? 2 : 1;  // pages of a tile
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t s_full[PAGED_WARPS][ST];
-    __shared__ int2 s_page[PAGED_WARPS][ST];   // a stage's page of each 16 keys, -1: none
+    __shared__ int32_t s_block[PAGED_WARPS][ST][HN];  // a stage's page * n_kv + head, -1: none
     __shared__ float s_m[PAGED_WARPS][PAGED_ROWS], s_l[PAGED_WARPS][PAGED_ROWS];
     __shared__ unsigned long long s_scan[PAGED_WARPS];
     __shared__ unsigned long long s_start;
@@ -138,10 +178,11 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
                                                 ~(uintptr_t)1023);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t g = lane >> 2, c = lane & 3u;  // the tile instructions' row and column group
-    const uint32_t shift = p.page_shift, passes = (p.group + PAGED_ROWS - 1) / PAGED_ROWS;
+    const uint32_t shift = SMALL ? 4u : p.page_shift;
+    const uint32_t passes = (p.group + PAGED_ROWS - 1) / PAGED_ROWS;
     const uint32_t per = (p.group + passes - 1) / passes;  // query heads a pass
     const uint32_t items = p.n_kv * passes;                // items of a sequence
-    const uint64_t b = blockIdx.x;
+    const uint32_t b = blockIdx.x;
     if (lane == 0)
         for (uint32_t s = 0; s < ST; ++s) mbar_init(&s_full[warp][s], 1);
     if (tid == 0) s_abort = 0;
@@ -149,40 +190,40 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
     pdl_launch_dependents();
     pdl_wait();
 
-    auto units_of = [&](uint32_t s) -> uint32_t {  // 0 for an empty or refused sequence
-        const int64_t n = __ldg(p.length + s);
+    auto units_of = [&](int64_t n) -> uint32_t {  // 0 for an empty or refused sequence
         return n <= 0 || n > ((int64_t)p.max_pages << shift)
                    ? 0u
                    : (uint32_t)((n + PAGED_UNIT - 1) / PAGED_UNIT);
     };
-    // rows of sequences without keys
-    for (uint32_t s = (uint32_t)b; s < p.n_seqs; s += gridDim.x) {
-        if (units_of(s) == 0u) {
-            if (tid == 0 && __ldg(p.length + s) != 0) atomicOr(p.status, WL_DEV_ERR_INDEX);
-            for (uint32_t i = tid; i < p.n_kv * p.group * D; i += PAGED_THREADS)
-                store_typed(p.out, p.out_type, s * p.out_stride + i, 0.0f);
-        }
-    }
+    auto units_at = [&](uint32_t s) { return units_of(__ldg(p.length + s)); };
     // all units, and the sequence in which this CTA's share begins
-    uint64_t total = 0;
+    const uint32_t mine = tid < p.n_seqs ? units_at(tid) : 0u;
+    uint64_t total;
     {
-        uint64_t mine = 0;
-        for (uint32_t s = tid; s < p.n_seqs; s += PAGED_THREADS) mine += units_of(s);
+        uint64_t sum = mine;
+        for (uint32_t s = tid + PAGED_THREADS; s < p.n_seqs; s += PAGED_THREADS) sum += units_at(s);
 #pragma unroll
-        for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-        if (lane == 0) s_scan[warp] = mine;
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) s_scan[warp] = sum;
         __syncthreads();
-        for (int w = 0; w < PAGED_WARPS; ++w) total += s_scan[w];
-        total *= items;
+        total = (s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3]) * items;
     }
-    const uint64_t N = min((uint64_t)gridDim.x, total);  // CTAs with a share, at least a unit each
-    if (b >= N) return;
-    const uint64_t begin = b * total / N, end = (b + 1) * total / N;
-    {
+    // N CTAs with a share: `extra` of them have quota + 1 units, the others quota (at least 1)
+    const uint32_t N = (uint32_t)min((uint64_t)gridDim.x, total);
+    const uint64_t quota = N ? div_fast(total, N) : 0u;
+    const uint32_t extra = (uint32_t)(total - quota * N);
+    const uint64_t begin = quota * b + min(b, extra), end = begin + quota + (b < extra);
+    auto cta_of = [&](uint64_t unit) -> uint32_t {
+        const uint64_t split = (quota + 1u) * extra;
+        if (quota >> 31) return (uint32_t)(unit < split ? unit / (quota + 1u) : extra + (unit - split) / quota);
+        return (uint32_t)(unit < split ? div_fast(unit, (uint32_t)quota + 1u)
+                                       : extra + div_fast(unit - split, (uint32_t)quota));
+    };
+    if (b < N) {
         uint64_t before = 0;
         for (uint32_t s0 = 0; s0 < p.n_seqs; s0 += PAGED_THREADS) {
             const uint32_t s = s0 + tid;
-            const uint64_t u = s < p.n_seqs ? (uint64_t)units_of(s) * items : 0u;
+            const uint64_t u = (uint64_t)(s0 == 0 ? mine : s < p.n_seqs ? units_at(s) : 0u) * items;
             uint64_t incl = u;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -193,6 +234,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
             if (lane == 31) s_scan[warp] = incl;
             __syncthreads();
             uint64_t sum = 0;
+#pragma unroll
             for (int w = 0; w < PAGED_WARPS; ++w) {
                 if (w == (int)warp) incl += before + sum;
                 sum += s_scan[w];
@@ -213,71 +255,96 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
     uint32_t seq = s_seq;
     uint64_t seq_unit = s_start;  // the sequence's first unit
     auto segment_at = [&](uint64_t at) {  // at < end, ascending from call to call
-        uint32_t nu = units_of(seq);
+        uint32_t n = (uint32_t)__ldg(p.length + seq), nu = units_of((int32_t)n);
         while (at >= seq_unit + (uint64_t)nu * items) {  // the next sequence with keys
             seq_unit += (uint64_t)nu * items;
             ++seq;
-            nu = units_of(seq);
+            n = (uint32_t)__ldg(p.length + seq);
+            nu = units_of((int32_t)n);
         }
         PagedSegment s;
-        const uint32_t item = (uint32_t)((at - seq_unit) / nu), pass = item % passes;
+        const uint32_t item = (uint32_t)div_fast(at - seq_unit, nu);
+        const uint32_t pass = passes == 1u ? 0u : item % passes;
         s.seq = seq;
-        s.h = item / passes;
+        s.h = passes == 1u ? item : item / passes;
         s.row0 = pass * per;
         s.rows = min(per, p.group - s.row0);
-        s.n = (uint32_t)__ldg(p.length + seq);
+        s.n = n;
         s.n_units = nu;
         s.item0 = seq_unit + (uint64_t)item * nu;
         s.u0 = (uint32_t)(at - s.item0);
         s.u1 = (uint32_t)(min(end, s.item0 + nu) - s.item0);
         return s;
     };
-    auto page_at = [&](const PagedSegment &s, uint32_t t) -> int32_t {  // of key t < n, -1 if refused
-        const int32_t page = __ldg(p.page_table + (size_t)s.seq * p.max_pages + (t >> shift));
-        if (page >= 0 && (uint32_t)page < p.n_pages) return page;
-        atomicOr(p.status, WL_DEV_ERR_INDEX);
-        return -1;
+    // table entries of this warp's tile of unit u: keys [u * UNIT + warp * TILE, + TILE);
+    // -1 where no key is.  Read ahead; checked when the tile is copied.
+    struct Pages {
+        int32_t id[HN];
     };
-    // pages of this warp's tile of unit u: keys [u * UNIT + warp * TILE, + TILE)
     auto pages_of = [&](const PagedSegment &s, uint32_t u) {
         const uint32_t t = u * PAGED_UNIT + warp * PAGED_TILE;
-        int2 r = make_int2(-1, -1);
-        if (t < s.n) r.x = r.y = page_at(s, t);
-        if (shift == 4u) r.y = t + 16u < s.n ? page_at(s, t + 16u) : -1;
+        const int32_t *row = p.page_table + (size_t)s.seq * p.max_pages + (t >> shift);
+        Pages r;
+#pragma unroll
+        for (int a = 0; a < HN; ++a) r.id[a] = t + 16u * a < s.n ? __ldg(row + a) : -1;
         return r;
     };
     uint8_t *ring = smem + warp * L::WARP;
     uint32_t issued = 0;  // (lane 0) ring entries filled
     // (lane 0) the tile of unit u into ring entry `entry`, each in turn
-    auto issue = [&](const PagedSegment &s, uint32_t u, uint32_t entry, int2 page) {
+    auto issue = [&](const PagedSegment &s, uint32_t u, uint32_t entry, Pages page) {
         issued = entry + 1u;
         const uint32_t st = entry % ST, t = u * PAGED_UNIT + warp * PAGED_TILE;
         uint8_t *dst = ring + st * L::STAGE;
         uint64_t *bar = &s_full[warp][st];
-        s_page[warp][st] = page;
-        if (shift != 4u) {
-            mbar_arrive_expect_tx(bar, page.x >= 0 ? L::STAGE : 0u);
-            if (page.x >= 0) {
-                const uint32_t row = (((uint32_t)page.x * p.n_kv + s.h) << shift) + (t & ((1u << shift) - 1u));
-                tma_load_2d_plain(dst, &maps.k, 0, row, bar);
-                tma_load_2d_plain(dst + L::HALF, &maps.v, 0, row, bar);
-            }
-        } else {
-            mbar_arrive_expect_tx(bar, ((page.x >= 0) + (page.y >= 0)) * (L::STAGE / 2u));
+        uint32_t bytes = 0;
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                const int32_t pg = a ? page.y : page.x;
-                if (pg >= 0) {
-                    const uint32_t row = ((uint32_t)pg * p.n_kv + s.h) << 4;
-                    tma_load_2d_plain(dst + a * (L::HALF / 2u), &maps.k, 0, row, bar);
-                    tma_load_2d_plain(dst + L::HALF + a * (L::HALF / 2u), &maps.v, 0, row, bar);
-                }
+        for (int a = 0; a < HN; ++a) {
+            const bool good = (uint32_t)page.id[a] < p.n_pages;  // negative ids are large ones
+            if (!good && t + 16u * a < s.n) atomicOr(p.status, WL_DEV_ERR_INDEX);
+            page.id[a] = good ? page.id[a] * (int32_t)p.n_kv + (int32_t)s.h : -1;
+            s_block[warp][st][a] = page.id[a];
+            bytes += good ? L::STAGE / HN : 0u;
+        }
+        mbar_arrive_expect_tx(bar, bytes);
+#pragma unroll
+        for (int a = 0; a < HN; ++a) {
+            if (page.id[a] >= 0) {
+                const uint32_t row = ((uint32_t)page.id[a] << shift) + (t & ((1u << shift) - 1u) & ~31u);
+                tma_load_2d_plain(dst + a * (L::HALF / HN), &maps.k, 0, row, bar);
+                tma_load_2d_plain(dst + L::HALF + a * (L::HALF / HN), &maps.v, 0, row, bar);
             }
         }
     };
+
+    uint64_t at = begin;
+    uint32_t it = 0;                     // ring entries consumed
+    PagedSegment sg;
+    if (b < N) {
+        sg = segment_at(at);
+        if (lane == 0) {
+            Pages first[ST];
+#pragma unroll
+            for (uint32_t i = 0; i < ST - 1u; ++i)
+                if (sg.u0 + i < sg.u1) first[i] = pages_of(sg, sg.u0 + i);
+#pragma unroll
+            for (uint32_t i = 0; i < ST - 1u; ++i)
+                if (sg.u0 + i < sg.u1) issue(sg, sg.u0 + i, it + i, first[i]);
+        }
+    }
+    // rows of sequences without keys
+    for (uint32_t s = b; s < p.n_seqs; s += gridDim.x) {
+        const int32_t n = __ldg(p.length + s);
+        if (units_of(n) == 0u) {
+            if (tid == 0 && n != 0) atomicOr(p.status, WL_DEV_ERR_INDEX);
+            for (uint32_t i = tid; i < p.n_kv * p.group * D; i += PAGED_THREADS)
+                store_typed(p.out, p.out_type, s * p.out_stride + i, 0.0f);
+        }
+    }
+    if (b >= N) return;
     // lane's places in a stage: keys' row g, 16-byte pieces of its four dimensions
     // groups; values' rows 2c, 2c + 1 (and 8 more, 16 more), its D / 8 dimensions
-    uint32_t koff[D / 64], voff[2];
+    uint32_t koff[KW], voff[2];
     if constexpr (D == 128) {
         koff[0] = g * 128u + (((2u * c) ^ g) << 4);
         koff[1] = g * 128u + (((2u * c + 1u) ^ g) << 4);
@@ -289,70 +356,58 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
         voff[1] = voff[0] + 64u;
     }
 
-    uint64_t at = begin;
-    uint32_t it = 0;                     // ring entries consumed
-    PagedSegment sg = segment_at(at);
-    if (lane == 0)
-        for (uint32_t i = 0; i < ST - 1u && sg.u0 + i < sg.u1; ++i)
-            issue(sg, sg.u0 + i, it + i, pages_of(sg, sg.u0 + i));
     bool ok = true;
     for (;;) {
         const uint32_t head = sg.h * p.group + sg.row0;
         // the entry that the joining of the segment before had used, and the pages
         // of the one after it
-        int2 ahead = make_int2(-1, -1);
+        Pages ahead;
         if (lane == 0) {
             if (sg.u0 + ST - 1u < sg.u1) issue(sg, sg.u0 + ST - 1u, it + ST - 1u, pages_of(sg, sg.u0 + ST - 1u));
             if (sg.u0 + ST < sg.u1) ahead = pages_of(sg, sg.u0 + ST);
         }
-        __syncwarp();
-        const float *ksh = p.ks + sg.h, *vsh = p.vs + sg.h;
-        auto scales = [&](uint32_t entry, int2 &page, float (&s)[4]) {
-            page = s_page[warp][entry % ST];
-            s[0] = page.x >= 0 ? __ldg(ksh + (size_t)page.x * p.n_kv) : 0.0f;
-            s[1] = page.x >= 0 ? __ldg(vsh + (size_t)page.x * p.n_kv) : 0.0f;
-            s[2] = s[0];
-            s[3] = s[1];
-            if (shift == 4u) {
-                s[2] = page.y >= 0 ? __ldg(ksh + (size_t)page.y * p.n_kv) : 0.0f;
-                s[3] = page.y >= 0 ? __ldg(vsh + (size_t)page.y * p.n_kv) : 0.0f;
-            }
-        };
-        int2 page;
-        float sc[4];
-        scales(it, page, sc);
-
         // the pass's query rows: row g as f16 parts hi (tile row g) and lo (row
         // g + 8) of q * 2^shift, its largest |q| brought to [2^13, 2^14)
         uint32_t qa[D / 16][4];
         float qf;  // scale * log2(e) * 2^-shift
         {
             float x[D / 4];
+#pragma unroll
+            for (int i = 0; i < D / 4; ++i) x[i] = 0.0f;
+            if (g < sg.rows)
+                load_row_part(p.q, p.type, sg.seq * p.q_stride + (size_t)(head + g) * D + c * (D / 4), x);
             float top = 0.0f;
 #pragma unroll
-            for (int j = 0; j < D / 16; ++j) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[4 * j + i] =
-                        g < sg.rows ? load_typed(p.q, p.type, sg.seq * p.q_stride + (size_t)(head + g) * D +
-                                                                  c * (D / 4) + 4 * j + i)
-                                    : 0.0f;
-                    top = fmaxf(top, fabsf(x[4 * j + i]));
-                }
-            }
+            for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(x[i]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int e = top > 0.0f && top < INFINITY ? ilogbf(top) : 0;
-            // 2^(13 - e) in two factors, each of them a float
-            const float f0 = ldexpf(1.0f, (13 - e) / 2), f1 = ldexpf(1.0f, (13 - e) - (13 - e) / 2);
-            qf = p.scale * 1.4426950408889634f * ldexpf(1.0f, (e - 13) / 2) *
-                 ldexpf(1.0f, (e - 13) - (e - 13) / 2);
+            // 2^(13 - e) for 2^e <= top < 2^(e + 1), in two factors that are floats;
+            // e kept so large that its opposite is one too
+            const int e = top > 0.0f && top < INFINITY
+                              ? max((int)(__float_as_uint(top) >> 23), 1) - 127 : 0;
+            const int s0 = (13 - e) / 2, s1 = 13 - e - s0;
+            const float f0 = __uint_as_float((uint32_t)(127 + s0) << 23);
+            const float f1 = __uint_as_float((uint32_t)(127 + s1) << 23);
+            qf = p.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - s0) << 23) *
+                 __uint_as_float((uint32_t)(127 - s1) << 23);
 #pragma unroll
             for (int j = 0; j < D / 16; ++j) {
                 split_f16(x[4 * j] * f0 * f1, x[4 * j + 1] * f0 * f1, qa[j][0], qa[j][1]);
                 split_f16(x[4 * j + 2] * f0 * f1, x[4 * j + 3] * f0 * f1, qa[j][2], qa[j][3]);
             }
         }
+        __syncwarp();
+        int32_t block[HN];
+        float ks[HN], vs[HN];
+        auto scales = [&](uint32_t entry, int32_t (&blk)[HN], float (&k)[HN], float (&v)[HN]) {
+#pragma unroll
+            for (int a = 0; a < HN; ++a) {
+                blk[a] = s_block[warp][entry % ST][a];
+                k[a] = blk[a] >= 0 ? __ldg(p.ks + blk[a]) : 0.0f;
+                v[a] = blk[a] >= 0 ? __ldg(p.vs + blk[a]) : 0.0f;
+            }
+        };
+        scales(it, block, ks, vs);
 
         float m = -INFINITY, l = 0.0f, vref = 0.0f;
         float o[NT][4];
@@ -362,41 +417,47 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
         for (uint32_t u = sg.u0; u < sg.u1; ++u, ++it) {
             const uint32_t t0 = u * PAGED_UNIT + warp * PAGED_TILE;
             const uint8_t *st = ring + (it % ST) * L::STAGE;
-            int2 page_next = make_int2(-1, -1);
-            float sc_next[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (u + 1 < sg.u1) scales(it + 1, page_next, sc_next);
+            int32_t block_next[HN];
+            float ks_next[HN], vs_next[HN];
+            if (u + 1 < sg.u1) scales(it + 1, block_next, ks_next, vs_next);
             ok = __all_sync(0xffffffffu, mbar_wait(&s_full[warp][it % ST], (it / ST) & 1u));
             if (!ok) break;
-            if (page.x >= 0 || page.y >= 0) {
+            if (block[0] >= 0 || block[HN - 1] >= 0) {
                 float s[4][4];
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
+                for (int t = 0; t < 4; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
 #pragma unroll
-                    for (int w = 0; w < D / 64; ++w) {
+                for (int w = 0; w < KW; ++w) {
+                    uint32_t x[4][4];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
                         const uint4 r = lds128(st + koff[w] + t * 8 * D);
-                        const uint32_t x[4] = {r.x ^ 0x80808080u, r.y ^ 0x80808080u, r.z ^ 0x80808080u,
-                                               r.w ^ 0x80808080u};
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            mma_f16(s[t], qa[4 * w + j], unbias(__byte_perm(x[j], EXP1024, 0x4140)),
-                                    unbias(__byte_perm(x[j], EXP1024, 0x4342)));
+                        x[t][0] = r.x ^ 0x80808080u;
+                        x[t][1] = r.y ^ 0x80808080u;
+                        x[t][2] = r.z ^ 0x80808080u;
+                        x[t][3] = r.w ^ 0x80808080u;
                     }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int t = 0; t < 4; ++t)
+                            mma_f16(s[t], qa[4 * w + j], unbias(__byte_perm(x[t][j], EXP1024, 0x4140)),
+                                    unbias(__byte_perm(x[t][j], EXP1024, 0x4342)));
                 }
                 // z in log2 units, keys 2c, 2c+1 of each 8
                 float z[4][2];
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
-                    const float f = qf * sc[t < 2 ? 0 : 2];
+                    const float f = qf * ks[SMALL ? t / 2 : 0];
                     z[t][0] = (s[t][0] + s[t][2]) * f;
                     z[t][1] = (s[t][1] + s[t][3]) * f;
                 }
-                if (t0 + PAGED_TILE > sg.n || page.x < 0 || page.y < 0) {  // keys that take no part
+                if (t0 + PAGED_TILE > sg.n || (SMALL && (block[0] | block[HN - 1]) < 0)) {  // not all take part
 #pragma unroll
                     for (int t = 0; t < 4; ++t)
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
-                            if (t0 + 8u * t + 2u * c + i >= sg.n || (t < 2 ? page.x : page.y) < 0)
+                            if (t0 + 8u * t + 2u * c + i >= sg.n || block[SMALL ? t / 2 : 0] < 0)
                                 z[t][i] = -INFINITY;
                 }
                 float top = -INFINITY;
@@ -404,7 +465,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
                 for (int t = 0; t < 4; ++t) top = fmaxf(top, fmaxf(z[t][0], z[t][1]));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float vtop = fmaxf(fabsf(sc[1]), fabsf(sc[3]));
+                const float vtop = fmaxf(fabsf(vs[0]), fabsf(vs[HN - 1]));
                 if (__any_sync(0xffffffffu, top > m) || vtop > vref) {
                     const float mn = fmaxf(m, top), vn = fmaxf(vref, vtop);
                     const float shrink = mn == -INFINITY ? 0.0f : ex2_approx(m - mn);
@@ -423,11 +484,11 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
                 // weights times 2^14, so that the f16 parts of small ones keep their bits,
                 // and relative to the largest scale of the values so far
                 const float base = 14.0f - (m == -INFINITY ? 0.0f : m);
-                const float r0 = sc[1] == 0.0f ? 0.0f : sc[1] / vref, r1 = sc[3] == 0.0f ? 0.0f : sc[3] / vref;
 #pragma unroll
                 for (int a = 0; a < 2; ++a) {
                     uint32_t w[4];
-                    const float r = a ? r1 : r0;
+                    const float va = vs[SMALL ? a : 0];
+                    const float r = va == vref ? 1.0f : va / vref;  // vref 0 only with va 0: scaled by 0 at the end
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const float e0 = ex2_approx(z[2 * a + i][0] + base);
@@ -474,9 +535,12 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
                 if (u + ST + 1u < sg.u1) ahead = pages_of(sg, u + ST + 1u);
             }
             __syncwarp();
-            page = page_next;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sc[i] = sc_next[i];
+            for (int a = 0; a < HN; ++a) {
+                block[a] = block_next[a];
+                ks[a] = ks_next[a];
+                vs[a] = vs_next[a];
+            }
         }
         if (!ok) {
             if (lane == 0) {
@@ -512,61 +576,94 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
         const bool stop = s_abort != 0u;  // a wait ran out: nothing more is read or written
         const bool whole = done.u0 == 0 && done.u1 == done.n_units;
         const size_t slot = (size_t)b * 2u + (done.u0 != 0 ? 0u : 1u);
-        if (!stop) {
-            for (uint32_t i = tid; i < done.rows * D; i += PAGED_THREADS) {
-                const uint32_t r = i / D, k = i % D;
-                float mx = -INFINITY;
+        // a warp takes a row, a lane D / 32 of its values k: dimensions (k % 8) * D / 8 + k / 8
+        constexpr int OV = D / 32;
+        auto write_row = [&](uint32_t r, const float (&acc)[OV], float sum) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const size_t to = done.seq * p.out_stride + (size_t)(head + r) * D;
 #pragma unroll
-                for (int w = 0; w < PAGED_WARPS; ++w) mx = fmaxf(mx, s_m[w][r]);
+            for (int i = 0; i < OV; ++i) {
+                const uint32_t k = lane * OV + i;
+                store_typed(p.out, p.out_type, to + (k & 7u) * (D / 8) + (k >> 3),
+                            sum == 0.0f ? 0.0f : acc[i] * inv);
+            }
+        };
+        if (!stop) {
+            for (uint32_t r = warp; r < done.rows; r += PAGED_WARPS) {
+                const float mx = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
                 const float ref = mx == -INFINITY ? 0.0f : mx;
-                float sum = 0.0f, acc = 0.0f;
+                float sum = 0.0f, acc[OV];
+#pragma unroll
+                for (int i = 0; i < OV; ++i) acc[i] = 0.0f;
 #pragma unroll
                 for (int w = 0; w < PAGED_WARPS; ++w) {
                     const float f = ex2_approx(s_m[w][r] - ref);
+                    const float *src = reinterpret_cast<const float *>(smem + w * L::WARP + free_at) + r * OP + lane * OV;
                     sum = fmaf(s_l[w][r], f, sum);
-                    acc = fmaf(reinterpret_cast<const float *>(smem + w * L::WARP + free_at)[r * OP + k], f, acc);
+#pragma unroll
+                    for (int i = 0; i < OV; ++i) acc[i] = fmaf(src[i], f, acc[i]);
                 }
                 if (whole) {
-                    const uint32_t d = (k & 7u) * (D / 8) + (k >> 3);
-                    store_typed(p.out, p.out_type, done.seq * p.out_stride + (size_t)(head + r) * D + d,
-                                sum == 0.0f ? 0.0f : acc / sum);
+                    write_row(r, acc, sum);
                 } else {
-                    po[(slot * PAGED_ROWS + r) * D + k] = acc;
-                    if (k == 0) ml[slot * PAGED_ROWS + r] = make_float2(mx, sum);
+#pragma unroll
+                    for (int i = 0; i < OV; ++i) po[(slot * PAGED_ROWS + r) * D + lane * OV + i] = acc[i];
+                    if (lane == 0) ml[slot * PAGED_ROWS + r] = make_float2(mx, sum);
                 }
             }
             if (!whole) {
                 // the CTAs that share the item: the last to arrive joins their parts in order
-                const uint32_t first = (uint32_t)(((done.item0 + 1) * N - 1) / total);
-                const uint32_t last = (uint32_t)(((done.item0 + done.n_units) * N - 1) / total);
-                __threadfence();
+                const uint32_t first = cta_of(done.item0), last = cta_of(done.item0 + done.n_units - 1u);
                 __syncthreads();
                 if (tid == 0) {
-                    const uint32_t before = atomicAdd(counters + first, 1u);
+                    uint32_t before;
+                    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
+                                 : "=r"(before)
+                                 : "l"(counters + first)
+                                 : "memory");
                     s_last = before == last - first;
                     if (s_last) counters[first] = 0u;
-                    __threadfence();
                 }
                 __syncthreads();
                 if (s_last) {
-                    for (uint32_t i = tid; i < done.rows * D; i += PAGED_THREADS) {
-                        const uint32_t r = i / D, k = i % D;
+                    for (uint32_t r = warp; r < done.rows; r += PAGED_WARPS) {
+                        auto part = [&](uint32_t x) { return ((size_t)x * 2u + (x == first)) * PAGED_ROWS + r; };
                         float mx = -INFINITY;
-                        for (uint32_t x = first; x <= last; ++x)
-                            mx = fmaxf(mx, __ldcg(&ml[((size_t)x * 2u + (x == first)) * PAGED_ROWS + r]).x);
+                        for (uint32_t x = first + lane; x <= last; x += 32u) mx = fmaxf(mx, __ldcg(&ml[part(x)]).x);
+#pragma unroll
+                        for (int q = 16; q; q >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, q));
                         const float ref = mx == -INFINITY ? 0.0f : mx;
-                        float sum = 0.0f, acc = 0.0f;
-#pragma unroll 4
-                        for (uint32_t x = first; x <= last; ++x) {
-                            const size_t y = ((size_t)x * 2u + (x == first)) * PAGED_ROWS + r;
-                            const float2 v = __ldcg(&ml[y]);
-                            const float f = ex2_approx(v.x - ref);
-                            sum = fmaf(v.y, f, sum);
-                            acc = fmaf(__ldcg(&po[y * D + k]), f, acc);
+                        float sum = 0.0f, acc[OV];
+#pragma unroll
+                        for (int i = 0; i < OV; ++i) acc[i] = 0.0f;
+                        for (uint32_t x0 = first; x0 <= last; x0 += 32u) {
+                            float f = 0.0f;
+                            if (x0 + lane <= last) {
+                                const float2 v = __ldcg(&ml[part(x0 + lane)]);
+                                f = ex2_approx(v.x - ref);
+                                sum = fmaf(v.y, f, sum);
+                            }
+                            const uint32_t count = min(32u, last - x0 + 1u);
+#pragma unroll 8
+                            for (uint32_t k = 0; k < count; ++k) {
+                                const float fk = __shfl_sync(0xffffffffu, f, k);
+                                const float *src = po + part(x0 + k) * D + lane * OV;
+                                if constexpr (OV == 4) {
+                                    const float4 v = __ldcg(reinterpret_cast<const float4 *>(src));
+                                    acc[0] = fmaf(v.x, fk, acc[0]);
+                                    acc[1] = fmaf(v.y, fk, acc[1]);
+                                    acc[2] = fmaf(v.z, fk, acc[2]);
+                                    acc[3] = fmaf(v.w, fk, acc[3]);
+                                } else {
+                                    const float2 v = __ldcg(reinterpret_cast<const float2 *>(src));
+                                    acc[0] = fmaf(v.x, fk, acc[0]);
+                                    acc[1] = fmaf(v.y, fk, acc[1]);
+                                }
+                            }
                         }
-                        const uint32_t d = (k & 7u) * (D / 8) + (k >> 3);
-                        store_typed(p.out, p.out_type, done.seq * p.out_stride + (size_t)(head + r) * D + d,
-                                    sum == 0.0f ? 0.0f : acc / sum);
+#pragma unroll
+                        for (int q = 16; q; q >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, q);
+                        write_row(r, acc, sum);
                     }
                 }
             }

@@ -287,12 +287,11 @@ int wl_dev_attn_decode_i8(const wl_kv_pages_i8 *cache, const wl_attn_decode *a, 
     p.workspace = a->workspace;
     const uint32_t ctas = std::min<uint32_t>((uint32_t)sm_count_for_launch() * PAGED_CTAS_PER_SM,
                                              PAGED_MAX_CTAS);
-    if (D == 64)
-        WL_CUDA(launch(attn_decode_i8_kernel<64>, dim3(ctas), dim3(PAGED_THREADS), PagedSmem<64>::DYN,
-                       (cudaStream_t)stream, true, maps, p));
-    else
-        WL_CUDA(launch(attn_decode_i8_kernel<128>, dim3(ctas), dim3(PAGED_THREADS), PagedSmem<128>::DYN,
-                       (cudaStream_t)stream, true, maps, p));
+    auto kernel = cache->page_size == 16
+                      ? (D == 64 ? attn_decode_i8_kernel<64, true> : attn_decode_i8_kernel<128, true>)
+                      : (D == 64 ? attn_decode_i8_kernel<64, false> : attn_decode_i8_kernel<128, false>);
+    WL_CUDA(launch(kernel, dim3(ctas), dim3(PAGED_THREADS), D == 64 ? PagedSmem<64>::DYN : PagedSmem<128>::DYN,
+                   (cudaStream_t)stream, true, maps, p));
     return WL_OK;
 }
 

@@ -171,8 +171,10 @@ int configure_kernels() {
                             (const void *)attn_gqa_batch_kernel<128, 2>,
                             (const void *)attn_gqa_batch_kernel<128, 3>,
                             (const void *)attn_gqa_batch_kernel<128, 4>,
-                            (const void *)attn_decode_i8_kernel<64>,
-                            (const void *)attn_decode_i8_kernel<128>,
+                            (const void *)attn_decode_i8_kernel<64, false>,
+                            (const void *)attn_decode_i8_kernel<64, true>,
+                            (const void *)attn_decode_i8_kernel<128, false>,
+                            (const void *)attn_decode_i8_kernel<128, true>,
                             (const void *)attn_prompt_kernel<__half, 64>,
                             (const void *)attn_prompt_kernel<__half, 128>,
                             (const void *)attn_prompt_kernel<__nv_bfloat16, 64>,
