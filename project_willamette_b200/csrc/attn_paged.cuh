@@ -50,12 +50,13 @@ constexpr int PAGED_THREADS = 128;
 constexpr int PAGED_WARPS = PAGED_THREADS / 32;
 constexpr int PAGED_TILE = 32;                           // keys of a warp's step
 constexpr int PAGED_UNIT = PAGED_TILE * PAGED_WARPS;     // keys of a CTA's step: the unit of work
-constexpr int PAGED_CTAS_PER_SM = 2;
+constexpr int PAGED_CTAS_PER_SM = 3;
 constexpr int PAGED_MAX_CTAS = 148 * PAGED_CTAS_PER_SM;
+constexpr int PAGED_JOIN = 16;                          // parts of a row read at once when joined
 constexpr int PAGED_ROWS = 8;                            // query heads of one pass over the keys
 
-// Caller's workspace: one arrival counter a CTA, then two partial results a
-// CTA (max and sum of each row, unnormalised output rows).
+// Caller's workspace: one arrival counter a CTA (zero between calls), then two partial
+// results a CTA (max and sum of each row, unnormalised output rows).
 __host__ __device__ constexpr size_t paged_ml_offset() { return (PAGED_MAX_CTAS * 4u + 255u) & ~255u; }
 __host__ __device__ constexpr size_t paged_o_offset() {
     return paged_ml_offset() + (size_t)PAGED_MAX_CTAS * 2u * PAGED_ROWS * 8u;
@@ -97,7 +98,7 @@ __device__ __forceinline__ void split_f16(float v0, float v1, uint32_t &hi, uint
 
 template <int D>
 struct PagedSmem {
-    static constexpr uint32_t STAGES = D == 128 ? 3 : 6;
+    static constexpr uint32_t STAGES = D == 128 ? 2 : 4;
     static constexpr uint32_t HALF = PAGED_TILE * D;   // a tile's keys; its values follow
     static constexpr uint32_t STAGE = 2u * HALF;
     static constexpr uint32_t WARP = STAGES * STAGE;
@@ -111,46 +112,111 @@ struct AttnDecodeMaps {
 
 // A contiguous run of one item's units, of one CTA.
 struct PagedSegment {
-    uint32_t seq, h, row0, rows;   // sequence, KV head, the pass's query heads within the group
-    uint32_t n, u0, u1, n_units;   // keys; units [u0, u1) of the item's n_units
-    uint64_t item0;                // the item's first unit
+    uint32_t seq, h, head, rows;  // sequence, KV head, the pass's first query head and their number
+    uint32_t n, u0, u1, n_units;  // keys; units [u0, u1) of the item's n_units
+    uint32_t first, last;         // CTAs that share the item
+    uint32_t valid;               // 0: the share is used up
 };
 
 __device__ __forceinline__ uint64_t div_fast(uint64_t a, uint32_t b) {
     return a >> 32 ? a / b : (uint64_t)((uint32_t)a / b);
 }
 
-// W = D / 4 consecutive elements as f32.
+// W consecutive elements, as they lie in memory (16-bit types fill half of raw)
+// and, once they are there, as f32.
 template <int W>
-__device__ __forceinline__ void load_row_part(const void *base, uint32_t type, size_t at, float (&x)[W]) {
-    if (type == 0u) {
-        const float4 *src = reinterpret_cast<const float4 *>(static_cast<const float *>(base) + at);
+__device__ __forceinline__ void load_row_part(const void *base, uint32_t type, size_t at, uint4 (&raw)[W / 4]) {
+    const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(base) + at * (type == 0u ? 4u : 2u));
 #pragma unroll
-        for (int i = 0; i < W / 4; ++i) {
-            const float4 v = __ldg(src + i);
-            x[4 * i] = v.x;
-            x[4 * i + 1] = v.y;
-            x[4 * i + 2] = v.z;
-            x[4 * i + 3] = v.w;
+    for (int i = 0; i < W / 4; ++i)
+        if (i < W / 8 || type == 0u) raw[i] = __ldg(src + i);
+}
+template <int W>
+__device__ __forceinline__ void prefetch_row_part(const void *base, uint32_t type, size_t at) {
+    const uint32_t size = type == 0u ? 4u : 2u;
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const uint8_t *>(base) + at * size));
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const uint8_t *>(base) + (at + W - 1) * size));
+}
+template <int W>
+__device__ __forceinline__ void row_part_f32(const uint4 (&raw)[W / 4], uint32_t type, float (&x)[W]) {
+#pragma unroll
+    for (int i = 0; i < W / 4; ++i) {
+        const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (type == 0u) {
+                x[4 * i + k] = __uint_as_float(u[k]);
+            } else if (i < W / 8) {
+                const float2 f = type == 1u ? __half22float2(*reinterpret_cast<const __half2 *>(&u[k]))
+                                            : make_float2(__uint_as_float(u[k] << 16),
+                                                          __uint_as_float(u[k] & 0xFFFF0000u));
+                x[8 * i + 2 * k] = f.x;
+                x[8 * i + 2 * k + 1] = f.y;
+            }
         }
-        return;
     }
-    const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + at);
-    uint4 raw[W / 8];
+}
+
+// A row's output from its sums.  A lane holds values k = lane * D / 32 + i, which
+// stand for dimensions (k % 8) * D / 8 + k / 8.
+template <int D>
+__device__ __forceinline__ void write_output_row(void *out, uint32_t out_type, size_t at,
+                                                 const float (&acc)[D / 32], float sum) {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-    for (int i = 0; i < W / 8; ++i) raw[i] = __ldg(src + i);
+    for (int i = 0; i < D / 32; ++i) {
+        const uint32_t k = (threadIdx.x & 31u) * (D / 32) + i;
+        store_typed(out, out_type, at + (k & 7u) * (D / 8) + (k >> 3), sum == 0.0f ? 0.0f : acc[i] * inv);
+    }
+}
+
+// One row of an item from its parts, of CTAs first, first + 1, ..., in that order; by a warp.
+template <int D>
+__device__ __forceinline__ void join_row(const void *workspace, uint32_t first, uint32_t count, uint32_t r, void *out,
+                                         uint32_t out_type, size_t at) {
+    constexpr int OV = D / 32, B = PAGED_JOIN;  // values a lane, parts in flight
+    const uint32_t lane = threadIdx.x & 31u;
+    const auto *ml = reinterpret_cast<const float2 *>(static_cast<const uint8_t *>(workspace) + paged_ml_offset());
+    const auto *po = reinterpret_cast<const float *>(static_cast<const uint8_t *>(workspace) + paged_o_offset());
+    auto part = [&](uint32_t x) { return ((first + x) * 2u + (x == 0u)) * PAGED_ROWS + r; };
+    float mx = -INFINITY, sum = 0.0f, acc[OV];
 #pragma unroll
-    for (int i = 0; i < W / 2; ++i) {
-        const uint32_t u = i % 4 == 0 ? raw[i / 4].x : i % 4 == 1 ? raw[i / 4].y : i % 4 == 2 ? raw[i / 4].z : raw[i / 4].w;
-        if (type == 1u) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u));
-            x[2 * i] = f.x;
-            x[2 * i + 1] = f.y;
-        } else {
-            x[2 * i] = __uint_as_float(u << 16);
-            x[2 * i + 1] = __uint_as_float(u & 0xFFFF0000u);
+    for (int i = 0; i < OV; ++i) acc[i] = 0.0f;
+#pragma unroll 1
+    for (uint32_t x0 = 0; x0 < count; x0 += B) {
+        float v[B][OV];
+        float2 e = make_float2(-INFINITY, 0.0f);
+        if (lane < B && x0 + lane < count) e = __ldcg(&ml[part(x0 + lane)]);
+#pragma unroll
+        for (int x = 0; x < B; ++x) {
+            const float *src = po + part(min(x0 + x, count - 1u)) * D + lane * OV;
+            if constexpr (OV == 4)
+                *reinterpret_cast<float4 *>(v[x]) = __ldcg(reinterpret_cast<const float4 *>(src));
+            else
+                *reinterpret_cast<float2 *>(v[x]) = __ldcg(reinterpret_cast<const float2 *>(src));
+        }
+        float top = e.x;
+#pragma unroll
+        for (int q = B / 2; q; q >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, q));
+        top = fmaxf(__shfl_sync(0xffffffffu, top, 0), mx);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        const float shrink = ex2_approx(mx - ref), f = ex2_approx(e.x - ref);
+        mx = top;
+        sum = fmaf(sum, shrink, lane < B ? e.y * f : 0.0f);
+#pragma unroll
+        for (int i = 0; i < OV; ++i) acc[i] *= shrink;
+#pragma unroll
+        for (int x = 0; x < B; ++x) {
+            const float fx = __shfl_sync(0xffffffffu, f, x);
+            if (x0 + x < count) {
+#pragma unroll
+                for (int i = 0; i < OV; ++i) acc[i] = fmaf(v[x][i], fx, acc[i]);
+            }
         }
     }
+#pragma unroll
+    for (int q = B / 2; q; q >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, q);
+    write_output_row<D>(out, out_type, at, acc, __shfl_sync(0xffffffffu, sum, 0));
 }
 
 // One CTA of PAGED_CTAS_PER_SM per SM takes an equal, contiguous share of all
@@ -169,10 +235,13 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
     constexpr int HN = SMALL ? 2 : 1;  // pages of a tile
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t s_full[PAGED_WARPS][ST];
+    __shared__ uint4 s_q[D / 16][32];  // query parts as the tile instructions take them
     __shared__ int32_t s_block[PAGED_WARPS][ST][HN];  // a stage's page * n_kv + head, -1: none
     __shared__ float s_m[PAGED_WARPS][PAGED_ROWS], s_l[PAGED_WARPS][PAGED_ROWS];
     __shared__ unsigned long long s_scan[PAGED_WARPS];
-    __shared__ unsigned long long s_start;
+    // the CTA's walk through its share, kept here by thread 0 so that it takes no registers
+    __shared__ PagedSegment s_sg[2];
+    __shared__ unsigned long long s_at, s_end, s_seq_unit;  // next unit, the share's end, s_seq's first unit
     __shared__ uint32_t s_seq, s_last, s_abort;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                 ~(uintptr_t)1023);
@@ -241,58 +310,65 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
             }
             if (u && incl > begin && incl - u <= begin) {
                 s_seq = s;
-                s_start = incl - u;
+                s_seq_unit = incl - u;
+                s_at = begin;
+                s_end = end;
             }
             before += sum;
             if (before > begin) break;  // the same for every thread
         }
         __syncthreads();
     }
-    auto *counters = static_cast<uint32_t *>(p.workspace);
     auto *ml = reinterpret_cast<float2 *>(static_cast<uint8_t *>(p.workspace) + paged_ml_offset());
     auto *po = reinterpret_cast<float *>(static_cast<uint8_t *>(p.workspace) + paged_o_offset());
 
-    uint32_t seq = s_seq;
-    uint64_t seq_unit = s_start;  // the sequence's first unit
-    auto segment_at = [&](uint64_t at) {  // at < end, ascending from call to call
-        uint32_t n = (uint32_t)__ldg(p.length + seq), nu = units_of((int32_t)n);
+    auto next_segment = [&](PagedSegment &s) {  // (thread 0)
+        const uint64_t at = s_at;
+        s.valid = at < s_end;
+        if (!s.valid) return;
+        uint32_t seq = s_seq;
+        uint64_t seq_unit = s_seq_unit;
+        int32_t n = __ldg(p.length + seq);
+        uint32_t nu = units_of(n);
         while (at >= seq_unit + (uint64_t)nu * items) {  // the next sequence with keys
             seq_unit += (uint64_t)nu * items;
-            ++seq;
-            n = (uint32_t)__ldg(p.length + seq);
-            nu = units_of((int32_t)n);
+            n = __ldg(p.length + ++seq);
+            nu = units_of(n);
         }
-        PagedSegment s;
         const uint32_t item = (uint32_t)div_fast(at - seq_unit, nu);
-        const uint32_t pass = passes == 1u ? 0u : item % passes;
+        const uint32_t h = passes == 1u ? item : item / passes, pass = item - h * passes;
+        const uint64_t item0 = seq_unit + (uint64_t)item * nu;
         s.seq = seq;
-        s.h = passes == 1u ? item : item / passes;
-        s.row0 = pass * per;
-        s.rows = min(per, p.group - s.row0);
-        s.n = n;
+        s.h = h;
+        s.head = h * p.group + pass * per;
+        s.rows = min(per, p.group - pass * per);
+        s.n = (uint32_t)n;
         s.n_units = nu;
-        s.item0 = seq_unit + (uint64_t)item * nu;
-        s.u0 = (uint32_t)(at - s.item0);
-        s.u1 = (uint32_t)(min(end, s.item0 + nu) - s.item0);
-        return s;
+        s.u0 = (uint32_t)(at - item0);
+        s.u1 = (uint32_t)(min((uint64_t)s_end, item0 + nu) - item0);
+        s.first = s.u0 == 0u ? b : cta_of(item0);
+        s.last = s.u1 == nu ? b : cta_of(item0 + nu - 1u);
+        s_seq = seq;
+        s_seq_unit = seq_unit;
+        s_at = item0 + s.u1;
     };
     // table entries of this warp's tile of unit u: keys [u * UNIT + warp * TILE, + TILE);
     // -1 where no key is.  Read ahead; checked when the tile is copied.
     struct Pages {
         int32_t id[HN];
     };
-    auto pages_of = [&](const PagedSegment &s, uint32_t u) {
+    auto pages_of = [&](uint32_t seq, uint32_t n, uint32_t u) {
         const uint32_t t = u * PAGED_UNIT + warp * PAGED_TILE;
-        const int32_t *row = p.page_table + (size_t)s.seq * p.max_pages + (t >> shift);
+        const int32_t *row = p.page_table + (size_t)seq * p.max_pages + (t >> shift);
         Pages r;
 #pragma unroll
-        for (int a = 0; a < HN; ++a) r.id[a] = t + 16u * a < s.n ? __ldg(row + a) : -1;
+        for (int a = 0; a < HN; ++a) r.id[a] = t + 16u * a < n ? __ldg(row + a) : -1;
         return r;
     };
     uint8_t *ring = smem + warp * L::WARP;
     uint32_t issued = 0;  // (lane 0) ring entries filled
     // (lane 0) the tile of unit u into ring entry `entry`, each in turn
-    auto issue = [&](const PagedSegment &s, uint32_t u, uint32_t entry, Pages page) {
+    auto issue = [&](uint32_t h, uint32_t n, uint32_t u, uint32_t entry, Pages page) {
         issued = entry + 1u;
         const uint32_t st = entry % ST, t = u * PAGED_UNIT + warp * PAGED_TILE;
         uint8_t *dst = ring + st * L::STAGE;
@@ -301,8 +377,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
 #pragma unroll
         for (int a = 0; a < HN; ++a) {
             const bool good = (uint32_t)page.id[a] < p.n_pages;  // negative ids are large ones
-            if (!good && t + 16u * a < s.n) atomicOr(p.status, WL_DEV_ERR_INDEX);
-            page.id[a] = good ? page.id[a] * (int32_t)p.n_kv + (int32_t)s.h : -1;
+            if (!good && t + 16u * a < n) atomicOr(p.status, WL_DEV_ERR_INDEX);
+            page.id[a] = good ? page.id[a] * (int32_t)p.n_kv + (int32_t)h : -1;
             s_block[warp][st][a] = page.id[a];
             bytes += good ? L::STAGE / HN : 0u;
         }
@@ -317,20 +393,30 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
         }
     };
 
-    uint64_t at = begin;
-    uint32_t it = 0;                     // ring entries consumed
-    PagedSegment sg;
-    if (b < N) {
-        sg = segment_at(at);
+    uint32_t it = 0;   // ring entries consumed
+    Pages ahead[2];    // (lane 0) table entries of the next two tiles to copy
+    // a segment's loads in one go: table entries, queries (into L1), then the first
+    // tiles' copies; one ring entry stays free for the joining of the segment before
+    auto begin_segment = [&](const PagedSegment &s) {
+        if (g < s.rows)
+            prefetch_row_part<D / 4>(p.q, p.type, s.seq * p.q_stride + (size_t)(s.head + g) * D + c * (D / 4));
         if (lane == 0) {
-            Pages first[ST];
+            const uint32_t seq = s.seq, h = s.h, n = s.n, u0 = s.u0, u1 = s.u1;
+            Pages first[ST + 1];
+#pragma unroll
+            for (uint32_t i = 0; i <= ST; ++i)
+                if (u0 + i < u1) first[i] = pages_of(seq, n, u0 + i);
 #pragma unroll
             for (uint32_t i = 0; i < ST - 1u; ++i)
-                if (sg.u0 + i < sg.u1) first[i] = pages_of(sg, sg.u0 + i);
-#pragma unroll
-            for (uint32_t i = 0; i < ST - 1u; ++i)
-                if (sg.u0 + i < sg.u1) issue(sg, sg.u0 + i, it + i, first[i]);
+                if (u0 + i < u1) issue(h, n, u0 + i, it + i, first[i]);
+            ahead[0] = first[ST - 1];
+            ahead[1] = first[ST];
         }
+    };
+    if (b < N) {
+        if (tid == 0) next_segment(s_sg[0]);
+        __syncthreads();
+        begin_segment(s_sg[0]);
     }
     // rows of sequences without keys
     for (uint32_t s = b; s < p.n_seqs; s += gridDim.x) {
@@ -357,32 +443,30 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
     }
 
     bool ok = true;
-    for (;;) {
-        const uint32_t head = sg.h * p.group + sg.row0;
-        // the entry that the joining of the segment before had used, and the pages
-        // of the one after it
-        Pages ahead;
-        if (lane == 0) {
-            if (sg.u0 + ST - 1u < sg.u1) issue(sg, sg.u0 + ST - 1u, it + ST - 1u, pages_of(sg, sg.u0 + ST - 1u));
-            if (sg.u0 + ST < sg.u1) ahead = pages_of(sg, sg.u0 + ST);
-        }
+    for (uint32_t turn = 0;; turn ^= 1u) {
+        const PagedSegment &sg = s_sg[turn];
+        const uint32_t seq = sg.seq, h = sg.h, n = sg.n, u1 = sg.u1;
+        // the entry that the joining of the segment before had used
+        if (lane == 0 && sg.u0 + ST - 1u < u1) issue(h, n, sg.u0 + ST - 1u, it + ST - 1u, ahead[0]);
+        if (tid == 0) next_segment(s_sg[turn ^ 1u]);
         // the pass's query rows: row g as f16 parts hi (tile row g) and lo (row
-        // g + 8) of q * 2^shift, its largest |q| brought to [2^13, 2^14)
-        uint32_t qa[D / 16][4];
+        // g + 8) of q * 2^shift, its largest |q| brought to [2^13, 2^14).  Kept in shared
+        // memory: in registers they would take the room of a third CTA's
         float qf;  // scale * log2(e) * 2^-shift
         {
-            float x[D / 4];
+            uint4 raw[D / 16];
 #pragma unroll
-            for (int i = 0; i < D / 4; ++i) x[i] = 0.0f;
+            for (int i = 0; i < D / 16; ++i) raw[i] = make_uint4(0, 0, 0, 0);
             if (g < sg.rows)
-                load_row_part(p.q, p.type, sg.seq * p.q_stride + (size_t)(head + g) * D + c * (D / 4), x);
+                load_row_part<D / 4>(p.q, p.type, seq * p.q_stride + (size_t)(sg.head + g) * D + c * (D / 4), raw);
+            float x[D / 4];
+            row_part_f32<D / 4>(raw, p.type, x);
             float top = 0.0f;
 #pragma unroll
             for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(x[i]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // 2^(13 - e) for 2^e <= top < 2^(e + 1), in two factors that are floats;
-            // e kept so large that its opposite is one too
+            // 2^(13 - e) for 2^e <= top < 2^(e + 1), in two factors that are floats
             const int e = top > 0.0f && top < INFINITY
                               ? max((int)(__float_as_uint(top) >> 23), 1) - 127 : 0;
             const int s0 = (13 - e) / 2, s1 = 13 - e - s0;
@@ -392,11 +476,14 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
                  __uint_as_float((uint32_t)(127 - s1) << 23);
 #pragma unroll
             for (int j = 0; j < D / 16; ++j) {
-                split_f16(x[4 * j] * f0 * f1, x[4 * j + 1] * f0 * f1, qa[j][0], qa[j][1]);
-                split_f16(x[4 * j + 2] * f0 * f1, x[4 * j + 3] * f0 * f1, qa[j][2], qa[j][3]);
+                if (j / (D / 64) != (int)warp) continue;  // a quarter of them by each warp
+                uint4 a;
+                split_f16(x[4 * j] * f0 * f1, x[4 * j + 1] * f0 * f1, a.x, a.y);
+                split_f16(x[4 * j + 2] * f0 * f1, x[4 * j + 3] * f0 * f1, a.z, a.w);
+                s_q[j][lane] = a;
             }
         }
-        __syncwarp();
+        __syncthreads();
         int32_t block[HN];
         float ks[HN], vs[HN];
         auto scales = [&](uint32_t entry, int32_t (&blk)[HN], float (&k)[HN], float (&v)[HN]) {
@@ -414,12 +501,12 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
 #pragma unroll
         for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 
-        for (uint32_t u = sg.u0; u < sg.u1; ++u, ++it) {
+        for (uint32_t u = sg.u0; u < u1; ++u, ++it) {
             const uint32_t t0 = u * PAGED_UNIT + warp * PAGED_TILE;
             const uint8_t *st = ring + (it % ST) * L::STAGE;
             int32_t block_next[HN];
             float ks_next[HN], vs_next[HN];
-            if (u + 1 < sg.u1) scales(it + 1, block_next, ks_next, vs_next);
+            if (u + 1 < u1) scales(it + 1, block_next, ks_next, vs_next);
             ok = __all_sync(0xffffffffu, mbar_wait(&s_full[warp][it % ST], (it / ST) & 1u));
             if (!ok) break;
             if (block[0] >= 0 || block[HN - 1] >= 0) {
@@ -438,11 +525,14 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
                         x[t][3] = r.w ^ 0x80808080u;
                     }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
+                    for (int j = 0; j < 4; ++j) {
+                        const uint4 a = lds128(&s_q[4 * w + j][lane]);
+                        const uint32_t qa[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
                         for (int t = 0; t < 4; ++t)
-                            mma_f16(s[t], qa[4 * w + j], unbias(__byte_perm(x[t][j], EXP1024, 0x4140)),
+                            mma_f16(s[t], qa, unbias(__byte_perm(x[t][j], EXP1024, 0x4140)),
                                     unbias(__byte_perm(x[t][j], EXP1024, 0x4342)));
+                    }
                 }
                 // z in log2 units, keys 2c, 2c+1 of each 8
                 float z[4][2];
@@ -452,12 +542,12 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
                     z[t][0] = (s[t][0] + s[t][2]) * f;
                     z[t][1] = (s[t][1] + s[t][3]) * f;
                 }
-                if (t0 + PAGED_TILE > sg.n || (SMALL && (block[0] | block[HN - 1]) < 0)) {  // not all take part
+                if (t0 + PAGED_TILE > n || (SMALL && (block[0] | block[HN - 1]) < 0)) {  // not all take part
 #pragma unroll
                     for (int t = 0; t < 4; ++t)
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
-                            if (t0 + 8u * t + 2u * c + i >= sg.n || block[SMALL ? t / 2 : 0] < 0)
+                            if (t0 + 8u * t + 2u * c + i >= n || block[SMALL ? t / 2 : 0] < 0)
                                 z[t][i] = -INFINITY;
                 }
                 float top = -INFINITY;
@@ -530,9 +620,9 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
                 }
             }
             __syncwarp();  // the entry is free again
-            if (lane == 0 && u + ST < sg.u1) {
-                issue(sg, u + ST, it + ST, ahead);
-                if (u + ST + 1u < sg.u1) ahead = pages_of(sg, u + ST + 1u);
+            if (lane == 0 && u + ST < u1) {
+                issue(h, n, u + ST, it + ST, ahead[1]);
+                if (u + ST + 1u < u1) ahead[1] = pages_of(seq, n, u + ST + 1u);
             }
             __syncwarp();
 #pragma unroll
@@ -547,15 +637,6 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
                 atomicOr(p.status - 1, WL_DEV_ERR_TIMEOUT);
                 *(volatile uint32_t *)&s_abort = 1u;
             }
-        }
-        // the next segment's first tiles into the entries that the joining does not use
-        at = sg.item0 + sg.u1;
-        const PagedSegment done = sg;
-        if (at < end) {
-            sg = segment_at(at);
-            if (ok && lane == 0)
-                for (uint32_t i = 0; i < ST - 1u && sg.u0 + i < sg.u1; ++i)
-                    issue(sg, sg.u0 + i, it + i, pages_of(sg, sg.u0 + i));
         }
         // the warps' shares of the segment, joined in warp order.  Output tile i,
         // column n stands for dimension n * D / 8 + i; kept at 8 i + n.
@@ -572,24 +653,16 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
             s_m[warp][g] = m;
             s_l[warp][g] = l * 6.103515625e-05f;
         }
+        // the next segment's first loads, beside this one's joining
+        if (ok && s_sg[turn ^ 1u].valid) begin_segment(s_sg[turn ^ 1u]);
         __syncthreads();
         const bool stop = s_abort != 0u;  // a wait ran out: nothing more is read or written
-        const bool whole = done.u0 == 0 && done.u1 == done.n_units;
-        const size_t slot = (size_t)b * 2u + (done.u0 != 0 ? 0u : 1u);
-        // a warp takes a row, a lane D / 32 of its values k: dimensions (k % 8) * D / 8 + k / 8
-        constexpr int OV = D / 32;
-        auto write_row = [&](uint32_t r, const float (&acc)[OV], float sum) {
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            const size_t to = done.seq * p.out_stride + (size_t)(head + r) * D;
-#pragma unroll
-            for (int i = 0; i < OV; ++i) {
-                const uint32_t k = lane * OV + i;
-                store_typed(p.out, p.out_type, to + (k & 7u) * (D / 8) + (k >> 3),
-                            sum == 0.0f ? 0.0f : acc[i] * inv);
-            }
-        };
         if (!stop) {
-            for (uint32_t r = warp; r < done.rows; r += PAGED_WARPS) {
+            constexpr int OV = D / 32;  // a warp takes a row, a lane D / 32 of its values
+            const bool whole = sg.u0 == 0 && u1 == sg.n_units;
+            const size_t to_row = seq * p.out_stride + (size_t)sg.head * D;
+            const uint32_t slot = (b * 2u + (sg.u0 != 0 ? 0u : 1u)) * PAGED_ROWS;
+            for (uint32_t r = warp; r < sg.rows; r += PAGED_WARPS) {
                 const float mx = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
                 const float ref = mx == -INFINITY ? 0.0f : mx;
                 float sum = 0.0f, acc[OV];
@@ -604,71 +677,32 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
                     for (int i = 0; i < OV; ++i) acc[i] = fmaf(src[i], f, acc[i]);
                 }
                 if (whole) {
-                    write_row(r, acc, sum);
+                    write_output_row<D>(p.out, p.out_type, to_row + (size_t)r * D, acc, sum);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < OV; ++i) po[(slot * PAGED_ROWS + r) * D + lane * OV + i] = acc[i];
-                    if (lane == 0) ml[slot * PAGED_ROWS + r] = make_float2(mx, sum);
+                    for (int i = 0; i < OV; ++i) po[(slot + r) * D + lane * OV + i] = acc[i];
+                    if (lane == 0) ml[slot + r] = make_float2(mx, sum);
                 }
             }
-            if (!whole) {
-                // the CTAs that share the item: the last to arrive joins their parts in order
-                const uint32_t first = cta_of(done.item0), last = cta_of(done.item0 + done.n_units - 1u);
+            if (!whole) {  // the last to arrive joins the item's parts
                 __syncthreads();
                 if (tid == 0) {
-                    uint32_t before;
+                    uint32_t *counter = static_cast<uint32_t *>(p.workspace) + sg.first, before;
                     asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
                                  : "=r"(before)
-                                 : "l"(counters + first)
+                                 : "l"(counter)
                                  : "memory");
-                    s_last = before == last - first;
-                    if (s_last) counters[first] = 0u;
+                    s_last = before == sg.last - sg.first;
+                    if (s_last) *counter = 0u;
                 }
                 __syncthreads();
-                if (s_last) {
-                    for (uint32_t r = warp; r < done.rows; r += PAGED_WARPS) {
-                        auto part = [&](uint32_t x) { return ((size_t)x * 2u + (x == first)) * PAGED_ROWS + r; };
-                        float mx = -INFINITY;
-                        for (uint32_t x = first + lane; x <= last; x += 32u) mx = fmaxf(mx, __ldcg(&ml[part(x)]).x);
-#pragma unroll
-                        for (int q = 16; q; q >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, q));
-                        const float ref = mx == -INFINITY ? 0.0f : mx;
-                        float sum = 0.0f, acc[OV];
-#pragma unroll
-                        for (int i = 0; i < OV; ++i) acc[i] = 0.0f;
-                        for (uint32_t x0 = first; x0 <= last; x0 += 32u) {
-                            float f = 0.0f;
-                            if (x0 + lane <= last) {
-                                const float2 v = __ldcg(&ml[part(x0 + lane)]);
-                                f = ex2_approx(v.x - ref);
-                                sum = fmaf(v.y, f, sum);
-                            }
-                            const uint32_t count = min(32u, last - x0 + 1u);
-#pragma unroll 8
-                            for (uint32_t k = 0; k < count; ++k) {
-                                const float fk = __shfl_sync(0xffffffffu, f, k);
-                                const float *src = po + part(x0 + k) * D + lane * OV;
-                                if constexpr (OV == 4) {
-                                    const float4 v = __ldcg(reinterpret_cast<const float4 *>(src));
-                                    acc[0] = fmaf(v.x, fk, acc[0]);
-                                    acc[1] = fmaf(v.y, fk, acc[1]);
-                                    acc[2] = fmaf(v.z, fk, acc[2]);
-                                    acc[3] = fmaf(v.w, fk, acc[3]);
-                                } else {
-                                    const float2 v = __ldcg(reinterpret_cast<const float2 *>(src));
-                                    acc[0] = fmaf(v.x, fk, acc[0]);
-                                    acc[1] = fmaf(v.y, fk, acc[1]);
-                                }
-                            }
-                        }
-#pragma unroll
-                        for (int q = 16; q; q >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, q);
-                        write_row(r, acc, sum);
-                    }
-                }
+                if (s_last)
+                    for (uint32_t r = warp; r < sg.rows; r += PAGED_WARPS)
+                        join_row<D>(p.workspace, sg.first, sg.last - sg.first + 1u, r, p.out, p.out_type,
+                                    to_row + (size_t)r * D);
             }
         }
-        if (at >= end || stop) break;
+        if (stop || !s_sg[turn ^ 1u].valid) break;
         // the joining's reads and writes of the ring come before the copy that follows
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
