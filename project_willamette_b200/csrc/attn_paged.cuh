@@ -114,8 +114,8 @@ struct AttnDecodeMaps {
 struct PagedSegment {
     uint32_t seq, h, head, rows;  // sequence, KV head, the pass's first query head and their number
     uint32_t n, u0, u1, n_units;  // keys; units [u0, u1) of the item's n_units
-    uint32_t first, last;         // CTAs that share the item
     uint32_t valid;               // 0: the share is used up
+    uint64_t item0;               // the item's place: one for its beginning, then one a unit
 };
 
 __device__ __forceinline__ uint64_t div_fast(uint64_t a, uint32_t b) {
@@ -235,14 +235,15 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
     constexpr int HN = SMALL ? 2 : 1;  // pages of a tile
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t s_full[PAGED_WARPS][ST];
-    __shared__ uint4 s_q[D / 16][32];  // query parts as the tile instructions take them
+    __shared__ uint4 s_q[2][D / 16][32];  // query parts as the tile instructions take them
     __shared__ int32_t s_block[PAGED_WARPS][ST][HN];  // a stage's page * n_kv + head, -1: none
     __shared__ float s_m[PAGED_WARPS][PAGED_ROWS], s_l[PAGED_WARPS][PAGED_ROWS];
     __shared__ unsigned long long s_scan[PAGED_WARPS];
-    // the CTA's walk through its share, kept here by thread 0 so that it takes no registers
-    __shared__ PagedSegment s_sg[2];
-    __shared__ unsigned long long s_at, s_end, s_seq_unit;  // next unit, the share's end, s_seq's first unit
-    __shared__ uint32_t s_seq, s_last, s_abort;
+    // the CTA's walk through its share, kept here so that it takes no registers: the segment
+    // before, this one and the next; next place, the share's end, s_seq's first place
+    __shared__ PagedSegment s_sg[3];
+    __shared__ unsigned long long s_at, s_end, s_seq_at, s_quota;
+    __shared__ uint32_t s_seq, s_extra, s_last, s_abort;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                 ~(uintptr_t)1023);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
@@ -264,35 +265,61 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
                    ? 0u
                    : (uint32_t)((n + PAGED_UNIT - 1) / PAGED_UNIT);
     };
-    auto units_at = [&](uint32_t s) { return units_of(__ldg(p.length + s)); };
-    // all units, and the sequence in which this CTA's share begins
-    const uint32_t mine = tid < p.n_seqs ? units_at(tid) : 0u;
+    // Places: each item has one for its beginning (its queries and its joining take about
+    // a unit's time) and one a unit.  All places, and the sequence where this CTA's begin
+    auto places_of = [&](int32_t n) -> uint32_t {
+        const uint32_t u = units_of(n);
+        return u ? u + 1u : 0u;
+    };
+    const int32_t my_n = tid < p.n_seqs ? __ldg(p.length + tid) : 0;
     uint64_t total;
     {
-        uint64_t sum = mine;
-        for (uint32_t s = tid + PAGED_THREADS; s < p.n_seqs; s += PAGED_THREADS) sum += units_at(s);
+        uint64_t sum = places_of(my_n);
+        for (uint32_t s = tid + PAGED_THREADS; s < p.n_seqs; s += PAGED_THREADS) sum += places_of(__ldg(p.length + s));
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) s_scan[warp] = sum;
         __syncthreads();
         total = (s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3]) * items;
     }
-    // N CTAs with a share: `extra` of them have quota + 1 units, the others quota (at least 1)
+    // the first N CTAs have a share: `extra` of them quota + 1 places, the others quota (at
+    // least 1)
     const uint32_t N = (uint32_t)min((uint64_t)gridDim.x, total);
-    const uint64_t quota = N ? div_fast(total, N) : 0u;
-    const uint32_t extra = (uint32_t)(total - quota * N);
-    const uint64_t begin = quota * b + min(b, extra), end = begin + quota + (b < extra);
-    auto cta_of = [&](uint64_t unit) -> uint32_t {
-        const uint64_t split = (quota + 1u) * extra;
-        if (quota >> 31) return (uint32_t)(unit < split ? unit / (quota + 1u) : extra + (unit - split) / quota);
-        return (uint32_t)(unit < split ? div_fast(unit, (uint32_t)quota + 1u)
-                                       : extra + div_fast(unit - split, (uint32_t)quota));
+    // the segment at place `at` < s_end, in or behind sequence seq, which has n keys and
+    // begins at place seq_at
+    auto next_segment = [&](PagedSegment &s, uint64_t at, uint32_t seq, uint64_t seq_at, int32_t n) {
+        uint32_t places = places_of(n);
+        while (at >= seq_at + (uint64_t)places * items) {  // the next sequence with keys
+            seq_at += (uint64_t)places * items;
+            n = __ldg(p.length + ++seq);
+            places = places_of(n);
+        }
+        const uint32_t item = (uint32_t)div_fast(at - seq_at, places);
+        const uint32_t h = passes == 1u ? item : item / passes, pass = item - h * passes;
+        const uint64_t item0 = seq_at + (uint64_t)item * places, stop = min((uint64_t)s_end, item0 + places);
+        s.seq = seq;
+        s.h = h;
+        s.head = h * p.group + pass * per;
+        s.rows = min(per, p.group - pass * per);
+        s.n = (uint32_t)n;
+        s.n_units = places - 1u;
+        s.u0 = at == item0 ? 0u : (uint32_t)(at - item0) - 1u;
+        s.u1 = (uint32_t)(stop - item0) - 1u;
+        s.item0 = item0;
+        s.valid = s.u0 < s.u1;  // not where the share ends with an item's beginning
+        s_seq = seq;
+        s_seq_at = seq_at;
+        s_at = stop;
     };
     if (b < N) {
+        const uint64_t quota = div_fast(total, N);
+        const uint32_t extra = (uint32_t)(total - quota * N);
+        const uint64_t begin = quota * b + min(b, extra);
         uint64_t before = 0;
         for (uint32_t s0 = 0; s0 < p.n_seqs; s0 += PAGED_THREADS) {
             const uint32_t s = s0 + tid;
-            const uint64_t u = (uint64_t)(s0 == 0 ? mine : s < p.n_seqs ? units_at(s) : 0u) * items;
+            const int32_t n = s0 == 0 ? my_n : s < p.n_seqs ? __ldg(p.length + s) : 0;
+            const uint64_t u = (uint64_t)places_of(n) * items;
             uint64_t incl = u;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -308,11 +335,11 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
                 if (w == (int)warp) incl += before + sum;
                 sum += s_scan[w];
             }
-            if (u && incl > begin && incl - u <= begin) {
-                s_seq = s;
-                s_seq_unit = incl - u;
-                s_at = begin;
-                s_end = end;
+            if (u && incl > begin && incl - u <= begin) {  // one thread
+                s_end = begin + quota + (b < extra);
+                s_quota = quota;
+                s_extra = extra;
+                next_segment(s_sg[0], begin, s, incl - u, n);
             }
             before += sum;
             if (before > begin) break;  // the same for every thread
@@ -322,36 +349,6 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
     auto *ml = reinterpret_cast<float2 *>(static_cast<uint8_t *>(p.workspace) + paged_ml_offset());
     auto *po = reinterpret_cast<float *>(static_cast<uint8_t *>(p.workspace) + paged_o_offset());
 
-    auto next_segment = [&](PagedSegment &s) {  // (thread 0)
-        const uint64_t at = s_at;
-        s.valid = at < s_end;
-        if (!s.valid) return;
-        uint32_t seq = s_seq;
-        uint64_t seq_unit = s_seq_unit;
-        int32_t n = __ldg(p.length + seq);
-        uint32_t nu = units_of(n);
-        while (at >= seq_unit + (uint64_t)nu * items) {  // the next sequence with keys
-            seq_unit += (uint64_t)nu * items;
-            n = __ldg(p.length + ++seq);
-            nu = units_of(n);
-        }
-        const uint32_t item = (uint32_t)div_fast(at - seq_unit, nu);
-        const uint32_t h = passes == 1u ? item : item / passes, pass = item - h * passes;
-        const uint64_t item0 = seq_unit + (uint64_t)item * nu;
-        s.seq = seq;
-        s.h = h;
-        s.head = h * p.group + pass * per;
-        s.rows = min(per, p.group - pass * per);
-        s.n = (uint32_t)n;
-        s.n_units = nu;
-        s.u0 = (uint32_t)(at - item0);
-        s.u1 = (uint32_t)(min((uint64_t)s_end, item0 + nu) - item0);
-        s.first = s.u0 == 0u ? b : cta_of(item0);
-        s.last = s.u1 == nu ? b : cta_of(item0 + nu - 1u);
-        s_seq = seq;
-        s_seq_unit = seq_unit;
-        s_at = item0 + s.u1;
-    };
     // table entries of this warp's tile of unit u: keys [u * UNIT + warp * TILE, + TILE);
     // -1 where no key is.  Read ahead; checked when the tile is copied.
     struct Pages {
@@ -413,11 +410,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
             ahead[1] = first[ST];
         }
     };
-    if (b < N) {
-        if (tid == 0) next_segment(s_sg[0]);
-        __syncthreads();
-        begin_segment(s_sg[0]);
-    }
+    if (b < N && s_sg[0].valid) begin_segment(s_sg[0]);
     // rows of sequences without keys
     for (uint32_t s = b; s < p.n_seqs; s += gridDim.x) {
         const int32_t n = __ldg(p.length + s);
@@ -427,7 +420,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
                 store_typed(p.out, p.out_type, s * p.out_stride + i, 0.0f);
         }
     }
-    if (b >= N) return;
+    if (b >= N || !s_sg[0].valid) return;
     // lane's places in a stage: keys' row g, 16-byte pieces of its four dimensions
     // groups; values' rows 2c, 2c + 1 (and 8 more, 16 more), its D / 8 dimensions
     uint32_t koff[KW], voff[2];
@@ -442,23 +435,22 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
         voff[1] = voff[0] + 64u;
     }
 
-    bool ok = true;
-    for (uint32_t turn = 0;; turn ^= 1u) {
-        const PagedSegment &sg = s_sg[turn];
-        const uint32_t seq = sg.seq, h = sg.h, n = sg.n, u1 = sg.u1;
-        // the entry that the joining of the segment before had used
-        if (lane == 0 && sg.u0 + ST - 1u < u1) issue(h, n, sg.u0 + ST - 1u, it + ST - 1u, ahead[0]);
-        if (tid == 0) next_segment(s_sg[turn ^ 1u]);
-        // the pass's query rows: row g as f16 parts hi (tile row g) and lo (row
-        // g + 8) of q * 2^shift, its largest |q| brought to [2^13, 2^14).  Kept in shared
-        // memory: in registers they would take the room of a third CTA's
-        float qf;  // scale * log2(e) * 2^-shift
-        {
+    bool ok = true, joining = false;
+    uint32_t free_at = 0;  // the ring entry that a segment's joining uses, the same in every warp
+    for (uint32_t turn = 0, side = 0;; side ^= 1u) {
+        const bool more = ok && s_sg[turn].valid;
+        float qf = 0.0f;  // scale * log2(e) * 2^-shift
+        if (more) {
+            // the pass's query rows: row g as f16 parts hi (tile row g) and lo (row
+            // g + 8) of q * 2^shift, its largest |q| brought to [2^13, 2^14).  Kept in
+            // shared memory: in registers they would take the room of a third CTA's
+            const PagedSegment &sg = s_sg[turn];
+            if (joining) begin_segment(sg);
             uint4 raw[D / 16];
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) raw[i] = make_uint4(0, 0, 0, 0);
             if (g < sg.rows)
-                load_row_part<D / 4>(p.q, p.type, seq * p.q_stride + (size_t)(sg.head + g) * D + c * (D / 4), raw);
+                load_row_part<D / 4>(p.q, p.type, sg.seq * p.q_stride + (size_t)(sg.head + g) * D + c * (D / 4), raw);
             float x[D / 4];
             row_part_f32<D / 4>(raw, p.type, x);
             float top = 0.0f;
@@ -480,10 +472,79 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
                 uint4 a;
                 split_f16(x[4 * j] * f0 * f1, x[4 * j + 1] * f0 * f1, a.x, a.y);
                 split_f16(x[4 * j + 2] * f0 * f1, x[4 * j + 3] * f0 * f1, a.z, a.w);
-                s_q[j][lane] = a;
+                s_q[side][j][lane] = a;
             }
         }
         __syncthreads();
+        const bool stop = s_abort != 0u;  // a wait ran out: nothing more is read or written
+        if (joining && !stop) {  // the warps' shares of the segment before, in warp order
+            constexpr int OV = D / 32;  // a warp takes a row, a lane D / 32 of its values
+            const PagedSegment &sg = s_sg[turn == 0u ? 2u : turn - 1u];
+            const bool whole = sg.u0 == 0 && sg.u1 == sg.n_units;
+            const size_t to_row = sg.seq * p.out_stride + (size_t)sg.head * D;
+            const uint32_t slot = (b * 2u + (sg.u0 != 0 ? 0u : 1u)) * PAGED_ROWS;
+            for (uint32_t r = warp; r < sg.rows; r += PAGED_WARPS) {
+                const float mx = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+                const float ref = mx == -INFINITY ? 0.0f : mx;
+                float sum = 0.0f, acc[OV];
+#pragma unroll
+                for (int i = 0; i < OV; ++i) acc[i] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < PAGED_WARPS; ++w) {
+                    const float f = ex2_approx(s_m[w][r] - ref);
+                    const float *src = reinterpret_cast<const float *>(smem + w * L::WARP + free_at) + r * OP + lane * OV;
+                    sum = fmaf(s_l[w][r], f, sum);
+#pragma unroll
+                    for (int i = 0; i < OV; ++i) acc[i] = fmaf(src[i], f, acc[i]);
+                }
+                if (whole) {
+                    write_output_row<D>(p.out, p.out_type, to_row + (size_t)r * D, acc, sum);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < OV; ++i) po[(slot + r) * D + lane * OV + i] = acc[i];
+                    if (lane == 0) ml[slot + r] = make_float2(mx, sum);
+                }
+            }
+            if (!whole) {  // the last CTA to arrive joins the item's parts
+                auto cta_of = [&](uint64_t place) -> uint32_t {
+                    const uint64_t quota = s_quota, border = (quota + 1u) * s_extra;
+                    if (quota >> 31)
+                        return (uint32_t)(place < border ? place / (quota + 1u) : s_extra + (place - border) / quota);
+                    return (uint32_t)(place < border ? div_fast(place, (uint32_t)quota + 1u)
+                                                     : s_extra + div_fast(place - border, (uint32_t)quota));
+                };
+                const uint32_t first = sg.u0 == 0u ? b : cta_of(sg.item0 + 1u);
+                const uint32_t last = sg.u1 == sg.n_units ? b : cta_of(sg.item0 + sg.n_units);
+                __syncthreads();
+                if (tid == 0) {
+                    uint32_t *counter = static_cast<uint32_t *>(p.workspace) + first, arrived;
+                    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
+                                 : "=r"(arrived)
+                                 : "l"(counter)
+                                 : "memory");
+                    s_last = arrived == last - first;
+                    if (s_last) *counter = 0u;
+                }
+                __syncthreads();
+                if (s_last)
+                    for (uint32_t r = warp; r < sg.rows; r += PAGED_WARPS)
+                        join_row<D>(p.workspace, first, last - first + 1u, r, p.out, p.out_type, to_row + (size_t)r * D);
+            }
+        }
+        if (stop || !more) break;
+        const uint32_t following = turn == 2u ? 0u : turn + 1u;
+        if (tid == PAGED_THREADS - 1) {
+            s_sg[following].valid = 0u;
+            if (s_at < s_end) next_segment(s_sg[following], s_at, s_seq, s_seq_at, __ldg(p.length + s_seq));
+        }
+        // the joining's reads and writes of the ring come before the copy that follows
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
+        const PagedSegment &sg = s_sg[turn];
+        const uint32_t seq = sg.seq, h = sg.h, n = sg.n, u1 = sg.u1;
+        // the entry that the joining of the segment before had used
+        if (lane == 0 && sg.u0 + ST - 1u < u1) issue(h, n, sg.u0 + ST - 1u, it + ST - 1u, ahead[0]);
+        __syncwarp();
         int32_t block[HN];
         float ks[HN], vs[HN];
         auto scales = [&](uint32_t entry, int32_t (&blk)[HN], float (&k)[HN], float (&v)[HN]) {
@@ -526,7 +587,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
                     }
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const uint4 a = lds128(&s_q[4 * w + j][lane]);
+                        const uint4 a = lds128(&s_q[side][4 * w + j][lane]);
                         const uint32_t qa[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
                         for (int t = 0; t < 4; ++t)
@@ -638,12 +699,12 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
                 *(volatile uint32_t *)&s_abort = 1u;
             }
         }
-        // the warps' shares of the segment, joined in warp order.  Output tile i,
-        // column n stands for dimension n * D / 8 + i; kept at 8 i + n.
+        // this warp's share of the segment.  Output tile i, column n stands for dimension
+        // n * D / 8 + i; kept at 8 i + n.
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         const float back = vref * 6.103515625e-05f;  // 2^-14
-        const uint32_t free_at = ((it + ST - 1u) % ST) * L::STAGE;  // the same in every warp
+        free_at = ((it + ST - 1u) % ST) * L::STAGE;
         float *so = reinterpret_cast<float *>(ring + free_at);
 #pragma unroll
         for (int i = 0; i < NT; ++i)
@@ -653,59 +714,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
             s_m[warp][g] = m;
             s_l[warp][g] = l * 6.103515625e-05f;
         }
-        // the next segment's first loads, beside this one's joining
-        if (ok && s_sg[turn ^ 1u].valid) begin_segment(s_sg[turn ^ 1u]);
-        __syncthreads();
-        const bool stop = s_abort != 0u;  // a wait ran out: nothing more is read or written
-        if (!stop) {
-            constexpr int OV = D / 32;  // a warp takes a row, a lane D / 32 of its values
-            const bool whole = sg.u0 == 0 && u1 == sg.n_units;
-            const size_t to_row = seq * p.out_stride + (size_t)sg.head * D;
-            const uint32_t slot = (b * 2u + (sg.u0 != 0 ? 0u : 1u)) * PAGED_ROWS;
-            for (uint32_t r = warp; r < sg.rows; r += PAGED_WARPS) {
-                const float mx = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-                const float ref = mx == -INFINITY ? 0.0f : mx;
-                float sum = 0.0f, acc[OV];
-#pragma unroll
-                for (int i = 0; i < OV; ++i) acc[i] = 0.0f;
-#pragma unroll
-                for (int w = 0; w < PAGED_WARPS; ++w) {
-                    const float f = ex2_approx(s_m[w][r] - ref);
-                    const float *src = reinterpret_cast<const float *>(smem + w * L::WARP + free_at) + r * OP + lane * OV;
-                    sum = fmaf(s_l[w][r], f, sum);
-#pragma unroll
-                    for (int i = 0; i < OV; ++i) acc[i] = fmaf(src[i], f, acc[i]);
-                }
-                if (whole) {
-                    write_output_row<D>(p.out, p.out_type, to_row + (size_t)r * D, acc, sum);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < OV; ++i) po[(slot + r) * D + lane * OV + i] = acc[i];
-                    if (lane == 0) ml[slot + r] = make_float2(mx, sum);
-                }
-            }
-            if (!whole) {  // the last to arrive joins the item's parts
-                __syncthreads();
-                if (tid == 0) {
-                    uint32_t *counter = static_cast<uint32_t *>(p.workspace) + sg.first, before;
-                    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
-                                 : "=r"(before)
-                                 : "l"(counter)
-                                 : "memory");
-                    s_last = before == sg.last - sg.first;
-                    if (s_last) *counter = 0u;
-                }
-                __syncthreads();
-                if (s_last)
-                    for (uint32_t r = warp; r < sg.rows; r += PAGED_WARPS)
-                        join_row<D>(p.workspace, sg.first, sg.last - sg.first + 1u, r, p.out, p.out_type,
-                                    to_row + (size_t)r * D);
-            }
-        }
-        if (stop || !s_sg[turn ^ 1u].valid) break;
-        // the joining's reads and writes of the ring come before the copy that follows
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncthreads();
+        joining = true;
+        turn = following;
     }
     // after a wait that ran out: (bounded) the copies still in flight land before
     // the CTA's shared memory goes
