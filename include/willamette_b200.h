@@ -393,7 +393,7 @@ typedef struct wl_kv_append {
     const int32_t *seq_start;  /* device, n_seqs + 1, ascending from 0 */
     const int32_t *position;   /* device, n_seqs: tokens in the cache before the call */
     const int32_t *page_table; /* device, n_seqs x max_pages */
-    const float *rope;         /* device, 8-byte aligned */
+    const float *rope;         /* device, 16-byte aligned */
     void *q_out, *k_out, *v_out;
     uint32_t type, out_type;   /* WL_GGML_F32, WL_GGML_F16 or WL_GGML_BF16 */
     uint32_t n_tokens, n_seqs, n_q_heads, max_pages;

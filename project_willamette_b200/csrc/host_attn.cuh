@@ -85,20 +85,34 @@ int attn_status(const char *op, uint32_t **status) {
     return WL_OK;
 }
 
-template <typename T>
-int launch_kv_append(const KvAppendParams &p, dim3 grid, cudaStream_t s) {
-    const uint32_t pieces = p.page_size * p.head_dim / 8u;  // 8-element pieces of a page and head
-    if (pieces <= 128)
-        WL_CUDA(launch(kv_append_kernel<T, 1, 128>, grid, dim3(256), 0, s, true, p));
-    else if (pieces <= 256)
-        WL_CUDA(launch(kv_append_kernel<T, 2, 128>, grid, dim3(256), 0, s, true, p));
-    else if (pieces <= 512)
-        WL_CUDA(launch(kv_append_kernel<T, 4, 128>, grid, dim3(256), 0, s, true, p));
-    else if (pieces <= 1024)
-        WL_CUDA(launch(kv_append_kernel<T, 8, 128>, grid, dim3(256), 0, s, true, p));
-    else
-        WL_CUDA(launch(kv_append_kernel<T, 8, 256>, grid, dim3(512), 0, s, true, p));
+template <typename T, int ITS, int RT, int HB, bool WHOLE>
+int launch_kv_append_as(KvAppendParams &p, cudaStream_t s) {
+    if (p.q) {
+        // one token a CTA while that leaves room on the SMs, then as many as six CTAs an SM need
+        const uint32_t ctas = 6u * (uint32_t)sm_count_for_launch();
+        p.q_block = std::min((p.n_tokens + ctas - 1u) / ctas, KV_APPEND_MAX_Q_BLOCK);
+        p.q_ctas = (p.n_tokens + p.q_block - 1u) / p.q_block;
+    }
+    const uint64_t units = (uint64_t)p.n_tokens / p.page_size + 2ull * p.n_seqs;
+    const uint64_t ctas = p.q_ctas + units * ((p.n_kv + HB - 1) / HB);
+    if (ctas > 0x7FFFFFFFull)
+        return fail(WL_ERR_INVALID_ARGUMENT, "rope_kv_append: %u tokens of %u sequences", p.n_tokens, p.n_seqs);
+    WL_CUDA(launch(kv_append_kernel<T, ITS, RT, HB, WHOLE>, dim3((uint32_t)ctas), dim3(2 * RT * HB), 0, s, true, p));
     return WL_OK;
+}
+
+// Threads by the rows of a page that a call can bring: a step's few tokens a sequence
+// fit one warp for K and one for V; whole pages of prompts get four 8-element pieces a
+// thread.  CTAs of 256 threads take as many heads as that leaves room for.
+template <typename T>
+int launch_kv_append(KvAppendParams &p, cudaStream_t s) {
+    const uint32_t rows = std::min(p.page_size, (p.n_tokens + p.n_seqs - 1u) / p.n_seqs);
+    const uint32_t pieces = rows * p.head_dim / 8u;
+    if (p.n_rot % 8u) return launch_kv_append_as<T, 2, 64, 2, false>(p, s);
+    if (pieces <= 32) return launch_kv_append_as<T, 1, 32, 4, true>(p, s);
+    if (pieces <= 256) return launch_kv_append_as<T, 4, 64, 2, true>(p, s);
+    if (pieces <= 512) return launch_kv_append_as<T, 4, 128, 1, true>(p, s);
+    return launch_kv_append_as<T, 4, 256, 1, true>(p, s);
 }
 
 // Tensor map of [n_tokens][heads][D] 16-bit rows `stride` elements apart: 128 tokens
@@ -175,8 +189,8 @@ int wl_dev_rope_kv_append_i8(const wl_kv_pages_i8 *cache, const wl_kv_append *a,
         return fail(WL_ERR_INVALID_ARGUMENT, "%s: q and q_out go together", op);
     if (!aligned16(a->q_out) || !aligned16(a->k_out) || !aligned16(a->v_out))
         return fail(WL_ERR_INVALID_ARGUMENT, "%s: q_out / k_out / v_out not 16-byte aligned", op);
-    if (a->n_rot && (!a->rope || (reinterpret_cast<uintptr_t>(a->rope) & 7u)))
-        return fail(WL_ERR_INVALID_ARGUMENT, "%s: rope is NULL or not 8-byte aligned", op);
+    if (a->n_rot && (!a->rope || !aligned16(a->rope)))
+        return fail(WL_ERR_INVALID_ARGUMENT, "%s: rope is NULL or not 16-byte aligned", op);
     if (a->max_pages == 0 || a->max_pages > 0x7FFFFFFFu / cache->page_size)
         return fail(WL_ERR_INVALID_ARGUMENT, "%s: max_pages %u", op, a->max_pages);
     KvAppendParams p;
@@ -211,14 +225,9 @@ int wl_dev_rope_kv_append_i8(const wl_kv_pages_i8 *cache, const wl_kv_append *a,
     p.n_rot = a->n_rot;
     p.rope_len = a->rope_len;
     p.rope_pairs = a->rope_pairs;
-    const uint64_t units = (uint64_t)a->n_tokens / cache->page_size + 2ull * a->n_seqs;
-    if (units > 0x7FFFFFFFull)
-        return fail(WL_ERR_INVALID_ARGUMENT, "%s: %u tokens of %u sequences", op, a->n_tokens,
-                    a->n_seqs);
-    const dim3 grid((uint32_t)units, KV);
-    if (type == 0) return launch_kv_append<float>(p, grid, (cudaStream_t)stream);
-    if (type == 1) return launch_kv_append<__half>(p, grid, (cudaStream_t)stream);
-    return launch_kv_append<__nv_bfloat16>(p, grid, (cudaStream_t)stream);
+    if (type == 0) return launch_kv_append<float>(p, (cudaStream_t)stream);
+    if (type == 1) return launch_kv_append<__half>(p, (cudaStream_t)stream);
+    return launch_kv_append<__nv_bfloat16>(p, (cudaStream_t)stream);
 }
 
 size_t wl_attn_decode_workspace_bytes(uint32_t n_seqs, uint32_t n_q_heads, uint32_t n_kv_heads,
