@@ -10,6 +10,7 @@
 #include <cuda.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "attn_paged.cuh"
 
@@ -102,6 +103,7 @@ __device__ __forceinline__ void prompt_row(const AttnPromptParams &p, int64_t be
 // not read what the mask leaves out.
 constexpr int PROMPT_THREADS = 320;
 constexpr int PROMPT_ROWS = 256;
+constexpr int PROMPT_POLY = 0;  // of 8 pairs of exponentials, those by polynomial
 
 template <int D>
 struct PromptSmem {
@@ -180,6 +182,39 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// The largest (smallest) of three, NaN if one of them is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// 2^x of two numbers at most 2^14 without the exponential unit: x = i + f, |f| <= 1/2,
+// 2^f by a polynomial of degree 5 (fitted here for the smallest largest relative error on
+// that interval, 2.4e-7 with its roundings), i added to the exponent.  Below -125 it
+// gives 2^-125; NaN is not kept.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+    constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: v + MAGIC holds rint(v) in its low bits
+    x.x = fmaxf(x.x, -125.0f);
+    x.y = fmaxf(x.y, -125.0f);
+    const float2 r = f2_add_rn(x, make_float2(MAGIC, MAGIC));
+    const float2 i = f2_add_rn(r, make_float2(-MAGIC, -MAGIC));
+    const float2 f = f2_fma_rn(i, make_float2(-1.0f, -1.0f), x);
+    float2 y = make_float2(0x1.5c08e6p-10f, 0x1.5c08e6p-10f);
+    y = f2_fma_rn(y, f, make_float2(0x1.3d0c54p-7f, 0x1.3d0c54p-7f));
+    y = f2_fma_rn(y, f, make_float2(0x1.c6b6e4p-5f, 0x1.c6b6e4p-5f));
+    y = f2_fma_rn(y, f, make_float2(0x1.ebf918p-3f, 0x1.ebf918p-3f));
+    y = f2_fma_rn(y, f, make_float2(0x1.62e428p-1f, 0x1.62e428p-1f));
+    y = f2_fma_rn(y, f, make_float2(0x1.000002p+0f, 0x1.000002p+0f));
+    return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(r.x) << 23)),
+                       __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(r.y) << 23)));
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack16(float a, float b);
 template <>
@@ -199,7 +234,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     using L = PromptSmem<D>;
     constexpr uint32_t ST = L::STAGES;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t q_full[2], kv_full[ST], kv_empty[ST], s_full[2], p_full[2], o_full[2];
+    __shared__ __align__(8) uint64_t q_full[2], kv_full[ST], kv_empty[ST], s_full[2], p_full[2][2], o_full[2];
     __shared__ uint32_t s_tmem, s_abort, s_seq;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                 ~(uintptr_t)1023);
@@ -218,7 +253,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         for (int i = 0; i < 2; ++i) {
             mbar_init(&q_full[i], 1);
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);  // one arrival a softmax warp
+            mbar_init(&p_full[i][0], 4);  // one arrival a softmax warp
+            mbar_init(&p_full[i][1], 4);
             mbar_init(&o_full[i], 1);
         }
         for (uint32_t s = 0; s < ST; ++s) {
@@ -312,12 +348,19 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
                 }
                 umma_commit(&s_full[t]);
             };
-            auto outputs = [&](uint32_t t, uint32_t it, bool add) {  // tile t: O += W V
+            // tile t: O += W V, for each half of the keys when its weights are there
+            auto outputs = [&](uint32_t t, uint32_t it, uint32_t j) {
                 const uint32_t v = stage(it);
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i)
-                    umma_f16_ts(tmem + 256u + t * 128u, tmem + t * 128u + i * 8u,
-                                umma_desc_mn_sw128(v + i * 2048u, 16384u), idesc_o, add || i != 0u);
+                for (uint32_t half = 0; half < 2; ++half) {
+                    if (!wait(&p_full[t][half], j & 1u)) return false;
+                    tc_fence_after();
+#pragma unroll
+                    for (uint32_t i = 4 * half; i < 4 * half + 4; ++i)
+                        umma_f16_ts(tmem + 256u + t * 128u, tmem + t * 128u + i * 8u,
+                                    umma_desc_mn_sw128(v + i * 2048u, 16384u), idesc_o, j != 0u || i != 0u);
+                }
+                return true;
             };
             // ring entries: K0, V0, K1, V1, ...
             bool ok = wait(&kv_full[0], 0);
@@ -338,9 +381,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
                 if (j + 1 < n_steps && !(ok = wait(&kv_full[k % ST], (k / ST) & 1u))) break;
                 for (uint32_t t = 0; t < 2; ++t) {
                     if (j >= steps[t]) continue;
-                    if (!(ok = wait(&p_full[t], j & 1u))) break;
-                    tc_fence_after();
-                    outputs(t, v, j != 0u);
+                    if (!(ok = outputs(t, v, j))) break;
                     if (j + 1 < steps[t])
                         scores(t, k);
                     else
@@ -365,38 +406,49 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         const uint32_t ts = tmem + lanes + t * 128u, to = tmem + lanes + 256u + t * 128u;
         const float sc = p.scale * 1.4426950408889634f;
         float m = 0.0f, l = 0.0f;  // m: the maximum in use, in log2 units
-        bool ok = true;
-        for (uint32_t j = 0; j < n; ++j) {
-            ok = __all_sync(0xffffffffu, wait(&s_full[t], j & 1u));
-            if (!ok) break;
-            tc_fence_after();
-            uint32_t s[128];
+        bool ok = true, fine = true;
+        // one step; DIAG: the last, where row r sees keys 0 .. r of the 128 (a code path of
+        // its own, so that the others carry no masks)
+        auto step = [&](uint32_t j, auto last) {
+            constexpr bool DIAG = decltype(last)::value;
+            // the scores 32 at a time, the second half first: the first stays in registers
+            // for the weights, the second is read again (all 128 in registers would leave
+            // too few for the exponentials to overlap)
+            uint32_t s[3][32];
+            float hi[4], lo[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) tmem_ld32(ts + 32u * i, s + 32 * i);
-            tmem_wait_ld();
-            const bool diagonal = j + 1 == n;
-            float hi = -INFINITY, lo = INFINITY;
-            if (diagonal) {
+            for (int q = 0; q < 4; ++q) hi[q] = -INFINITY, lo[q] = INFINITY;
 #pragma unroll
-                for (int i = 0; i < 128; ++i) {
-                    if ((uint32_t)i <= r) {
-                        hi = fmaxf(hi, __uint_as_float(s[i]));
-                        lo = fminf(lo, __uint_as_float(s[i]));
+            for (int half = 1; half >= 0; --half) {
+                tmem_ld32(ts + 64u * half, s[0]);
+                tmem_ld32(ts + 64u * half + 32u, s[1]);
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    auto score = [&](int i) { return __uint_as_float(s[c][i]); };
+                    if constexpr (DIAG) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            if ((uint32_t)(64 * half + 32 * c + i) <= r) {
+                                hi[i & 3] = max3_nan(hi[i & 3], score(i), score(i));
+                                lo[i & 3] = min3_nan(lo[i & 3], score(i), score(i));
+                            }
+                        }
+                    } else if (sc >= 0.0f) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2)
+                            hi[(i / 2) & 3] = max3_nan(hi[(i / 2) & 3], score(i), score(i + 1));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2)
+                            lo[(i / 2) & 3] = min3_nan(lo[(i / 2) & 3], score(i), score(i + 1));
                     }
                 }
-            } else if (sc >= 0.0f) {
-                float h4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int i = 0; i < 128; i += 8)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        h4[q] = fmaxf(fmaxf(h4[q], __uint_as_float(s[i + q])), __uint_as_float(s[i + q + 4]));
-                hi = fmaxf(fmaxf(h4[0], h4[1]), fmaxf(h4[2], h4[3]));
-            } else {
-#pragma unroll
-                for (int i = 0; i < 128; ++i) lo = fminf(lo, __uint_as_float(s[i]));
             }
-            const float top = sc >= 0.0f ? hi * sc : lo * sc;
+            float top = sc >= 0.0f ? max3_nan(max3_nan(hi[0], hi[1], hi[2]), hi[3], hi[3])
+                                   : min3_nan(min3_nan(lo[0], lo[1], lo[2]), lo[3], lo[3]);
+            top *= sc;
+            fine = fine && top < INFINITY;  // NaN or infinite scores: the row is computed again
             if (j == 0) {
                 m = top;
             } else if (__any_sync(0xffffffffu, top > m + 8.0f)) {
@@ -415,25 +467,50 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
                 }
             }
             const float base = 6.0f - (m == -INFINITY ? 0.0f : m);
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+            auto weigh = [&](uint32_t (&v)[32], uint32_t (&w)[32], int chunk) {  // 32 scores to 16 pairs of weights
 #pragma unroll
-            for (int i = 0; i < 128; i += 2) {
-                float a = ex2_approx(fmaf(__uint_as_float(s[i]), sc, base));
-                float b = ex2_approx(fmaf(__uint_as_float(s[i + 1]), sc, base));
-                if (diagonal) {
-                    a = (uint32_t)i <= r ? a : 0.0f;
-                    b = (uint32_t)(i + 1) <= r ? b : 0.0f;
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 x = f2_fma_rn(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])),
+                                               make_float2(sc, sc), make_float2(base, base));
+                    float2 e = (i / 2) % 8 < PROMPT_POLY ? ex2_poly(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                    if constexpr (DIAG) {
+                        e.x = (uint32_t)(32 * chunk + i) <= r ? e.x : 0.0f;
+                        e.y = (uint32_t)(32 * chunk + i + 1) <= r ? e.y : 0.0f;
+                    }
+                    sum[(i / 2) & 1] = f2_add_rn(sum[(i / 2) & 1], e);
+                    w[16 * (chunk & 1) + i / 2] = pack16<T>(e.x, e.y);
                 }
-                sum[(i / 2) & 3] += a + b;
-                s[i / 2] = pack16<T>(a, b);
-            }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tmem_st32(ts, s);
-            tmem_st32(ts + 32u, s + 32);
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[t]);
+            };
+            auto hand_over = [&](const uint32_t (&w)[32], int half) {
+                tmem_st32(ts + 32u * half, w);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[t][half]);
+            };
+            uint32_t w[32];
+            tmem_ld32(ts + 64u, s[2]);
+            weigh(s[0], w, 0);
+            weigh(s[1], w, 1);
+            tmem_wait_ld();
+            tmem_ld32(ts + 96u, s[0]);
+            hand_over(w, 0);
+            weigh(s[2], w, 2);
+            tmem_wait_ld();
+            weigh(s[0], w, 3);
+            hand_over(w, 1);
+            sum[0] = f2_add_rn(sum[0], sum[1]);
+            l += sum[0].x + sum[0].y;
+        };
+        for (uint32_t j = 0; j < n; ++j) {
+            ok = __all_sync(0xffffffffu, wait(&s_full[t], j & 1u));
+            if (!ok) break;
+            tc_fence_after();
+            if (j + 1 < n)
+                step(j, std::false_type());
+            else
+                step(j, std::true_type());
         }
         if (n) {
             if (ok) ok = __all_sync(0xffffffffu, wait(&o_full[t], 0));
@@ -442,7 +519,6 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
                 const int64_t row = begin + row0 + t * 128 + r;
                 const bool mine = row0 + t * 128 + r < len;
                 const float inv = 1.0f / l;
-                bool fine = true;
                 const size_t at = (size_t)row * p.out_stride + (size_t)head * D;
 #pragma unroll 1
                 for (int i = 0; i < D; i += 32) {
