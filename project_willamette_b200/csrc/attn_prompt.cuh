@@ -84,32 +84,40 @@ __device__ __forceinline__ void prompt_row(const AttnPromptParams &p, int64_t be
 }
 
 // ------------------------------------------------------------------ tensor cores
-// A CTA takes 256 rows of one head as two tiles of 128, and goes through the
-// keys 128 at a time.  Tensor memory (512 columns): scores of both tiles (128
-// f32 columns each; the weights overwrite them as 16-bit pairs) and both
-// outputs (D f32 columns each).
-//   warps 0-3, 4-7  softmax of tile 0 / 1, one thread a row: scores to
-//                   registers, row maximum, weights 2^(z - m + 6) back as 16-bit;
-//                   the output is rescaled only when the maximum has risen by more
-//                   than 2^8 over the one in use (weights then stay below 2^14);
-//   warp 8          TMA: queries, then keys and values through a ring;
-//   warp 9          MMA (one thread): weights x values of step j, then queries x keys
-//                   of step j + 1, for one tile and the other in turn, so that one
-//                   tile's softmax runs beside the other tile's products.
-// A commit on the scores of step j + 1 covers the earlier product into the
-// output as well, so who reads those scores may also rescale the output.
-// The masked part of a product is 0 x v, which is NaN where v is not finite:
-// a row whose output is not finite is computed again by prompt_row, which does
-// not read what the mask leaves out.
-constexpr int PROMPT_THREADS = 320;
-constexpr int PROMPT_ROWS = 256;
-constexpr int PROMPT_POLY = 0;  // of 8 pairs of exponentials, those by polynomial
+// A CTA takes 128 rows of one head and goes through the keys 128 at a time; two CTAs
+// share an SM, so that one's softmax runs beside the other's products.  Tensor memory
+// (256 columns a CTA): scores (128 f32 columns; the weights overwrite them as 16-bit
+// pairs) and output (D f32 columns).
+//   warps 0-3  softmax, one thread a row: scores to registers, row maximum, weights
+//              2^(z - m + 6) back as 16-bit, by halves; the output is rescaled only when
+//              the maximum has risen by more than 2^8 over the one in use (weights then
+//              stay below 2^14);
+//   warp 4     TMA: queries, then keys and values through a ring;
+//   warp 5     MMA (one thread): weights x values of step j, then queries x keys of step
+//              j + 1, with nothing between them (a commit there cost a tenth of the time).
+// The commit on the scores of step j + 1 covers the product into the output before it,
+// so who reads those scores may also rescale the output.
+// The masked part of a product is 0 x v, which is NaN where v is not finite: a row whose
+// scores or output are not finite is computed again by prompt_row, which does not read
+// what the mask leaves out.
+// What bounds it at D = 128: an SM's step of 128 x 128 takes 1090 cycles of products (64
+// to 70 an MMA, whose N = 64 costs as much as N = 128) and 1030 of exponentials (16 a
+// cycle), but a softmax warp needs 2200 from its scores to its last weights, and the next
+// scores are another 1000 away; two CTAs cover each other's waits to about 1850 a step.
+// Measured beside it: two tiles in one CTA of 10 warps (1 x 512 tokens of 20 heads 16.6
+// against 14.3 us, 32 x 256 72 against 62, 2 x 4096 198 against 187); 64-key steps with
+// two score buffers (763 against 600 us at 2 x 8k); weights through shared memory, so
+// that the next scores come beside the softmax (589 against 581); a part of the
+// exponentials by polynomial (4 to 20 % slower: the issue slots are what is short).
+constexpr int PROMPT_THREADS = 192;
+constexpr uint32_t PROMPT_ROWS = 128;
+constexpr uint32_t PROMPT_COLUMNS = 256;  // of tensor memory
 
 template <int D>
-struct PromptSmem {
-    static constexpr uint32_t TILE = 128u * D * 2u;      // 128 rows of queries, keys or values
-    static constexpr uint32_t STAGES = D == 128 ? 5 : 8;
-    static constexpr size_t DYN = (2 + STAGES) * TILE + 1024;  // + alignment slack
+struct PromptShape {
+    static constexpr uint32_t TILE = PROMPT_ROWS * D * 2u;  // 128 rows of queries, keys or values
+    static constexpr uint32_t STAGES = D == 128 ? 2 : 4;
+    static constexpr size_t DYN = (1 + STAGES) * TILE + 1024;  // + alignment slack
 };
 
 struct AttnPromptMaps {
@@ -194,27 +202,6 @@ __device__ __forceinline__ float min3_nan(float a, float b, float c) {
     return d;
 }
 
-// 2^x of two numbers at most 2^14 without the exponential unit: x = i + f, |f| <= 1/2,
-// 2^f by a polynomial of degree 5 (fitted here for the smallest largest relative error on
-// that interval, 2.4e-7 with its roundings), i added to the exponent.  Below -125 it
-// gives 2^-125; NaN is not kept.
-__device__ __forceinline__ float2 ex2_poly(float2 x) {
-    constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: v + MAGIC holds rint(v) in its low bits
-    x.x = fmaxf(x.x, -125.0f);
-    x.y = fmaxf(x.y, -125.0f);
-    const float2 r = f2_add_rn(x, make_float2(MAGIC, MAGIC));
-    const float2 i = f2_add_rn(r, make_float2(-MAGIC, -MAGIC));
-    const float2 f = f2_fma_rn(i, make_float2(-1.0f, -1.0f), x);
-    float2 y = make_float2(0x1.5c08e6p-10f, 0x1.5c08e6p-10f);
-    y = f2_fma_rn(y, f, make_float2(0x1.3d0c54p-7f, 0x1.3d0c54p-7f));
-    y = f2_fma_rn(y, f, make_float2(0x1.c6b6e4p-5f, 0x1.c6b6e4p-5f));
-    y = f2_fma_rn(y, f, make_float2(0x1.ebf918p-3f, 0x1.ebf918p-3f));
-    y = f2_fma_rn(y, f, make_float2(0x1.62e428p-1f, 0x1.62e428p-1f));
-    y = f2_fma_rn(y, f, make_float2(0x1.000002p+0f, 0x1.000002p+0f));
-    return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(r.x) << 23)),
-                       __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(r.y) << 23)));
-}
-
 template <typename T>
 __device__ __forceinline__ uint32_t pack16(float a, float b);
 template <>
@@ -229,13 +216,14 @@ __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float a, float b) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(PROMPT_THREADS, 1)
+__global__ void __launch_bounds__(PROMPT_THREADS, 2)
     attn_prompt_kernel(const __grid_constant__ AttnPromptMaps maps, const AttnPromptParams p) {
-    using L = PromptSmem<D>;
-    constexpr uint32_t ST = L::STAGES;
+    using L = PromptShape<D>;
+    constexpr uint32_t ST = L::STAGES, TMA_WARP = 4, MMA_WARP = 5;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t q_full[2], kv_full[ST], kv_empty[ST], s_full[2], p_full[2][2], o_full[2];
-    __shared__ uint32_t s_tmem, s_abort, s_seq;
+    __shared__ __align__(8) uint64_t q_full, kv_full[ST], kv_empty[ST], s_full, p_full[2], o_full;
+    __shared__ uint32_t s_tmem, s_abort;
+    __shared__ SeqExtent s_extent;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                 ~(uintptr_t)1023);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
@@ -243,20 +231,18 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     const uint32_t heads = p.n_kv * p.group, head = blockIdx.x % heads;
     const uint32_t unit = (gridDim.x - 1u - blockIdx.x) / heads;
 
-    if (warp == 9) {
+    if (warp == MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                          smem_u32(&s_tmem)),
-                     "r"(512u));
+                     "r"(PROMPT_COLUMNS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     if (tid == 0) {
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&q_full[i], 1);
-            mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i][0], 4);  // one arrival a softmax warp
-            mbar_init(&p_full[i][1], 4);
-            mbar_init(&o_full[i], 1);
-        }
+        mbar_init(&q_full, 1);
+        mbar_init(&s_full, 1);
+        mbar_init(&p_full[0], 4);  // one arrival a softmax warp
+        mbar_init(&p_full[1], 4);
+        mbar_init(&o_full, 1);
         for (uint32_t s = 0; s < ST; ++s) {
             mbar_init(&kv_full[s], 1);
             mbar_init(&kv_empty[s], 1);
@@ -264,30 +250,27 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         s_abort = 0;
         fence_mbar_init();
     }
+    if (warp == TMA_WARP && lane < 3u) {
+        const CUtensorMap *map = lane == 0u ? &maps.q : lane == 1u ? &maps.k : &maps.v;
+        asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+    }
     pdl_launch_dependents();
     pdl_wait();
-    if (warp == 8) {
-        const uint32_t s = find_seq(p.seq_start, p.n_seqs, PROMPT_ROWS, 1u, unit, lane);
-        if (lane == 0) s_seq = s;
+    if (warp == TMA_WARP) {
+        const SeqExtent e = find_extent(p.seq_start, nullptr, p.n_seqs, PROMPT_ROWS, 1u, unit, lane);
+        if (lane == 0) s_extent = e;
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
 
-    // this CTA's rows: [row0, row0 + 256) of the sequence, where there are any
-    const uint32_t seq = s_seq;
-    const int64_t begin = __ldg(p.seq_start + seq), stop = __ldg(p.seq_start + seq + 1);
+    // this CTA's rows: [row0, row0 + 128) of the sequence, where there are any
+    const int64_t begin = s_extent.begin, stop = s_extent.end, len = stop - begin;
     const bool bad = begin < 0 || stop < begin || stop > (int64_t)p.n_tokens;
     if (bad && tid == 0) atomicOr(p.status, WL_DEV_ERR_INDEX);
-    const int64_t len = stop - begin;
-    const int64_t row0 = ((int64_t)unit - (begin / PROMPT_ROWS + (int64_t)seq)) * PROMPT_ROWS;
-    uint32_t steps[2] = {0u, 0u};  // 128-key steps of each tile
-    if (!bad && row0 >= 0) {
-        if (row0 < len) steps[0] = (uint32_t)(row0 / 128) + 1u;
-        if (row0 + 128 < len) steps[1] = steps[0] + 1u;
-    }
-    const uint32_t n_steps = max(steps[0], steps[1]);
+    const int64_t row0 = ((int64_t)unit - (begin / PROMPT_ROWS + (int64_t)s_extent.seq)) * PROMPT_ROWS;
+    const uint32_t n = !bad && row0 >= 0 && row0 < len ? (uint32_t)(row0 / PROMPT_ROWS) + 1u : 0u;  // steps
 
     auto aborted = [&]() { return *(volatile uint32_t *)&s_abort != 0u; };
     auto wait = [&](uint64_t *bar, uint32_t parity) {  // false: the wait ran out, here or elsewhere
@@ -303,10 +286,12 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         }
         return true;
     };
+    auto wait_all = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
 
-    if (warp == 8) {
-        if (lane == 0 && n_steps) {
-            const uint32_t h = head / p.group, z0 = (uint32_t)(begin + row0);
+    if (n == 0u) {
+        // no rows
+    } else if (warp == TMA_WARP) {
+        if (lane == 0) {
             auto load_tile = [&](uint8_t *dst, const CUtensorMap *map, uint32_t y, uint32_t z, uint64_t *bar) {
                 mbar_arrive_expect_tx(bar, L::TILE);
 #pragma unroll
@@ -316,94 +301,72 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
             auto load_kv = [&](const CUtensorMap *map, uint32_t j) {
                 const uint32_t s = it % ST;
                 if (it >= ST && !wait(&kv_empty[s], (it / ST - 1u) & 1u)) return false;
-                load_tile(smem + (2u + s) * L::TILE, map, h, (uint32_t)begin + j * 128u, &kv_full[s]);
+                load_tile(smem + (1u + s) * L::TILE, map, head / p.group, (uint32_t)begin + j * 128u, &kv_full[s]);
                 ++it;
                 return true;
             };
-            load_tile(smem, &maps.q, head, z0, &q_full[0]);
-            bool ok = load_kv(&maps.k, 0);
-            if (steps[1]) load_tile(smem + L::TILE, &maps.q, head, z0 + 128u, &q_full[1]);
-            for (uint32_t j = 0; ok && j < n_steps; ++j) {
-                if (j) ok = load_kv(&maps.k, j);
-                if (ok) ok = load_kv(&maps.v, j);
-            }
+            load_tile(smem, &maps.q, head, (uint32_t)(begin + row0), &q_full);
+            bool ok = true;
+            for (uint32_t j = 0; ok && j < n; ++j) ok = load_kv(&maps.k, j) && load_kv(&maps.v, j);
             // (bounded) the last copies land before the CTA's shared memory goes
-            (void)mbar_wait(&q_full[0], 0);
-            if (steps[1]) (void)mbar_wait(&q_full[1], 0);
+            (void)mbar_wait(&q_full, 0);
             for (uint32_t k = it > ST ? it - ST : 0; k < it; ++k)
                 (void)mbar_wait(&kv_full[k % ST], (k / ST) & 1u);
         }
-    } else if (warp == 9) {
-        if (lane == 0 && n_steps) {
-            const uint32_t bf = sizeof(T) == 2 && pack16<T>(1.0f, 0.0f) == 0x3F80u;
+    } else if (warp == MMA_WARP) {
+        if (lane == 0) {
+            const uint32_t base = smem_u32(smem);
+            const uint32_t bf = pack16<T>(1.0f, 0.0f) == 0x3F80u;
             const uint32_t idesc_s = umma_idesc_f16(bf, 0u, 128u), idesc_o = umma_idesc_f16(bf, 1u, D);
-            auto stage = [&](uint32_t it) { return smem_u32(smem + (2u + it % ST) * L::TILE); };
-            auto scores = [&](uint32_t t, uint32_t it) {  // tile t: S = Q K^T, keys of ring entry it
-                const uint32_t q = smem_u32(smem + t * L::TILE), k = stage(it);
+            uint32_t freed = 0;  // ring entries (K0, V0, K1, V1, ...) whose reading is committed
+            auto entry = [&](uint32_t it) { return base + (1u + it % ST) * L::TILE; };
+            auto loaded = [&](uint32_t it) { return wait(&kv_full[it % ST], (it / ST) & 1u); };
+            auto free_next = [&]() { umma_commit(&kv_empty[freed++ % ST]); };
+            auto scores = [&](uint32_t it) {  // S = Q K^T
+                const uint32_t k = entry(it);
 #pragma unroll
                 for (uint32_t i = 0; i < (uint32_t)D / 16; ++i) {
                     const uint32_t off = (i / 4u) * 16384u + (i % 4u) * 32u;
-                    umma_f16_ss(tmem + t * 128u, umma_desc_sw128(q + off), umma_desc_sw128(k + off), idesc_s,
-                                i != 0u);
+                    umma_f16_ss(tmem, umma_desc_sw128(base + off), umma_desc_sw128(k + off), idesc_s, i != 0u);
                 }
-                umma_commit(&s_full[t]);
+                umma_commit(&s_full);
             };
-            // tile t: O += W V, for each half of the keys when its weights are there
-            auto outputs = [&](uint32_t t, uint32_t it, uint32_t j) {
-                const uint32_t v = stage(it);
+            bool ok = loaded(0) && wait(&q_full, 0);
+            if (ok) {
+                tc_fence_after();
+                scores(0);
+                free_next();
+            }
+            for (uint32_t j = 0; ok && j < n; ++j) {
+                const uint32_t v = 2u * j + 1u, k = v + 1u;
+                // all that the step needs before its weights, so that nothing comes between
+                // the two products
+                if (!(ok = loaded(v) && (j + 1 >= n || loaded(k)))) break;
 #pragma unroll
-                for (uint32_t half = 0; half < 2; ++half) {
-                    if (!wait(&p_full[t][half], j & 1u)) return false;
+                for (uint32_t half = 0; half < 2; ++half) {  // O += W V, each half when its weights are there
+                    ok = ok && wait(&p_full[half], j & 1u);
+                    if (!ok) break;
                     tc_fence_after();
 #pragma unroll
                     for (uint32_t i = 4 * half; i < 4 * half + 4; ++i)
-                        umma_f16_ts(tmem + 256u + t * 128u, tmem + t * 128u + i * 8u,
-                                    umma_desc_mn_sw128(v + i * 2048u, 16384u), idesc_o, j != 0u || i != 0u);
-                }
-                return true;
-            };
-            // ring entries: K0, V0, K1, V1, ...
-            bool ok = wait(&kv_full[0], 0);
-            uint32_t issued = 0;  // committed ring entries, for the drain
-            for (uint32_t t = 0; ok && t < 2; ++t) {
-                if (!steps[t]) continue;
-                if (!(ok = wait(&q_full[t], 0))) break;
-                tc_fence_after();
-                scores(t, 0);
-            }
-            if (ok) {
-                umma_commit(&kv_empty[0]);
-                issued = 1;
-            }
-            for (uint32_t j = 0; ok && j < n_steps; ++j) {
-                const uint32_t v = 2u * j + 1u, k = v + 1u;
-                if (!(ok = wait(&kv_full[v % ST], (v / ST) & 1u))) break;
-                if (j + 1 < n_steps && !(ok = wait(&kv_full[k % ST], (k / ST) & 1u))) break;
-                for (uint32_t t = 0; t < 2; ++t) {
-                    if (j >= steps[t]) continue;
-                    if (!(ok = outputs(t, v, j))) break;
-                    if (j + 1 < steps[t])
-                        scores(t, k);
-                    else
-                        umma_commit(&o_full[t]);
+                        umma_f16_ts(tmem + 128u, tmem + i * 8u, umma_desc_mn_sw128(entry(v) + i * 2048u, 16384u),
+                                    idesc_o, j != 0u || i != 0u);
                 }
                 if (!ok) break;
-                umma_commit(&kv_empty[v % ST]);
-                issued = v + 1;
-                if (j + 1 < n_steps) {
-                    umma_commit(&kv_empty[k % ST]);
-                    issued = k + 1;
-                }
+                if (j + 1 < n)
+                    scores(k);
+                else
+                    umma_commit(&o_full);
+                free_next();
+                if (j + 1 < n) free_next();
             }
             // (bounded) every committed product is done before tensor memory goes
-            for (uint32_t k = issued > ST ? issued - ST : 0; k < issued; ++k)
+            for (uint32_t k = freed > ST ? freed - ST : 0; k < freed; ++k)
                 (void)mbar_wait(&kv_empty[k % ST], (k / ST) & 1u);
         }
     } else {
-        const uint32_t t = warp >> 2, r = (warp & 3u) * 32u + lane;  // tile, row in the tile
-        const uint32_t n = steps[t];
-        const uint32_t lanes = ((warp & 3u) * 32u) << 16;
-        const uint32_t ts = tmem + lanes + t * 128u, to = tmem + lanes + 256u + t * 128u;
+        const uint32_t r = tid;  // row in the tile
+        const uint32_t ts = tmem + ((warp * 32u) << 16), to = ts + 128u;
         const float sc = p.scale * 1.4426950408889634f;
         float m = 0.0f, l = 0.0f;  // m: the maximum in use, in log2 units
         bool ok = true, fine = true;
@@ -473,7 +436,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
                 for (int i = 0; i < 32; i += 2) {
                     const float2 x = f2_fma_rn(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])),
                                                make_float2(sc, sc), make_float2(base, base));
-                    float2 e = (i / 2) % 8 < PROMPT_POLY ? ex2_poly(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                    float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
                     if constexpr (DIAG) {
                         e.x = (uint32_t)(32 * chunk + i) <= r ? e.x : 0.0f;
                         e.y = (uint32_t)(32 * chunk + i + 1) <= r ? e.y : 0.0f;
@@ -487,7 +450,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[t][half]);
+                if (lane == 0) mbar_arrive(&p_full[half]);
             };
             uint32_t w[32];
             tmem_ld32(ts + 64u, s[2]);
@@ -504,7 +467,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
             l += sum[0].x + sum[0].y;
         };
         for (uint32_t j = 0; j < n; ++j) {
-            ok = __all_sync(0xffffffffu, wait(&s_full[t], j & 1u));
+            ok = wait_all(&s_full, j & 1u);
             if (!ok) break;
             tc_fence_after();
             if (j + 1 < n)
@@ -512,44 +475,41 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
             else
                 step(j, std::true_type());
         }
-        if (n) {
-            if (ok) ok = __all_sync(0xffffffffu, wait(&o_full[t], 0));
-            if (ok) {
-                tc_fence_after();
-                const int64_t row = begin + row0 + t * 128 + r;
-                const bool mine = row0 + t * 128 + r < len;
-                const float inv = 1.0f / l;
-                const size_t at = (size_t)row * p.out_stride + (size_t)head * D;
+        if (ok && wait_all(&o_full, 0)) {
+            tc_fence_after();
+            const int64_t row = begin + row0 + r;
+            const bool mine = row0 + r < len;
+            const float inv = 1.0f / l;
+            const size_t at = (size_t)row * p.out_stride + (size_t)head * D;
 #pragma unroll 1
-                for (int i = 0; i < D; i += 32) {
-                    uint32_t o[32];
-                    tmem_ld32(to + i, o);
-                    tmem_wait_ld();
+            for (int i = 0; i < D; i += 32) {
+                uint32_t o[32];
+                tmem_ld32(to + i, o);
+                tmem_wait_ld();
 #pragma unroll
-                    for (int k = 0; k < 32; k += 8) {
-                        float x[8];
+                for (int k = 0; k < 32; k += 8) {
+                    float x[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            x[e] = __uint_as_float(o[k + e]) * inv;
-                            fine = fine && fabsf(x[e]) < INFINITY;
-                        }
-                        if (mine) store8(p.out, p.out_type, at + i + k, x);
+                    for (int e = 0; e < 8; ++e) {
+                        x[e] = __uint_as_float(o[k + e]) * inv;
+                        fine = fine && fabsf(x[e]) < INFINITY;
                     }
+                    if (mine) store8(p.out, p.out_type, at + i + k, x);
                 }
-                uint32_t again = __ballot_sync(0xffffffffu, mine && !fine);
-                while (again) {
-                    const uint32_t k = __ffs(again) - 1u;
-                    again &= again - 1u;
-                    prompt_row<T, D>(p, begin, row - r + (warp & 3u) * 32u + k, head, lane);
-                }
+            }
+            uint32_t again = __ballot_sync(0xffffffffu, mine && !fine);
+            while (again) {
+                const uint32_t k = __ffs(again) - 1u;
+                again &= again - 1u;
+                prompt_row<T, D>(p, begin, row - lane + k, head, lane);
             }
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == MMA_WARP) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(PROMPT_COLUMNS));
     }
 }
 

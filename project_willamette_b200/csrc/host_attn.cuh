@@ -140,16 +140,16 @@ int launch_attn_prompt(const AttnPromptParams &p, uint32_t D, cudaStream_t s) {
         (rc = encode_heads(enc, &maps.k, p.k, p.n_tokens, p.n_kv, D, p.k_stride)) ||
         (rc = encode_heads(enc, &maps.v, p.v, p.n_tokens, p.n_kv, D, p.v_stride)))
         return rc;
-    // sequence s owns the units [seq_start[s] / 256 + s, ...), at least as many as it needs
+    // sequence s owns the units [seq_start[s] / 128 + s, ...), at least as many as it needs
     const uint64_t ctas = ((uint64_t)p.n_tokens / PROMPT_ROWS + p.n_seqs) * p.n_kv * p.group;
     if (ctas > 0x7FFFFFFFull)
         return fail(WL_ERR_INVALID_ARGUMENT, "attn_prompt: %u tokens of %u sequences with %u heads",
                     p.n_tokens, p.n_seqs, p.n_kv * p.group);
     const dim3 grid((uint32_t)ctas), block(PROMPT_THREADS);
     if (D == 64)
-        WL_CUDA(launch(attn_prompt_kernel<T, 64>, grid, block, PromptSmem<64>::DYN, s, true, maps, p));
+        WL_CUDA(launch(attn_prompt_kernel<T, 64>, grid, block, PromptShape<64>::DYN, s, true, maps, p));
     else
-        WL_CUDA(launch(attn_prompt_kernel<T, 128>, grid, block, PromptSmem<128>::DYN, s, true, maps, p));
+        WL_CUDA(launch(attn_prompt_kernel<T, 128>, grid, block, PromptShape<128>::DYN, s, true, maps, p));
     return WL_OK;
 }
 

@@ -256,7 +256,8 @@ __device__ __forceinline__ uint32_t find_seq(const int32_t *seq_start, uint32_t 
     return lo;
 }
 
-// As find_seq, with the sequence's first and last token and the tokens before it.
+// As find_seq, with the sequence's first and last token and (position not NULL) the tokens
+// before it.
 struct SeqExtent {
     uint32_t seq;
     int32_t begin, end, before;
@@ -265,7 +266,7 @@ __device__ __forceinline__ SeqExtent find_extent(const int32_t *seq_start, const
                                                  uint32_t size, uint32_t extra, uint32_t u, uint32_t lane) {
     uint32_t lo = 0, n = n_seqs;
     SeqExtent e = {0u, 0, 0, 0};
-    if (n == 1u) e = {0u, __ldg(seq_start), __ldg(seq_start + 1), __ldg(position)};
+    if (n == 1u) e = {0u, __ldg(seq_start), __ldg(seq_start + 1), position ? __ldg(position) : 0};
     while (n > 1u) {
         const uint32_t step = (n + 31u) / 32u, s = lo + lane * step;
         bool below = lane * step < n;
@@ -274,7 +275,7 @@ __device__ __forceinline__ SeqExtent find_extent(const int32_t *seq_start, const
             a = __ldg(seq_start + s);
             if (step == 1u) {  // the last step: what the lane that it ends at needs is loaded beside
                 b = __ldg(seq_start + s + 1u);
-                before = __ldg(position + s);
+                if (position) before = __ldg(position + s);
             }
             below = a >= 0 && (uint64_t)((uint32_t)a / size) + (uint64_t)extra * s <= u;
         }
@@ -285,7 +286,7 @@ __device__ __forceinline__ SeqExtent find_extent(const int32_t *seq_start, const
             e = {lo, __shfl_sync(0xffffffffu, a, last), __shfl_sync(0xffffffffu, b, last),
                  __shfl_sync(0xffffffffu, before, last)};
         else if (n == 1u)
-            e = {lo, __ldg(seq_start + lo), __ldg(seq_start + lo + 1u), __ldg(position + lo)};
+            e = {lo, __ldg(seq_start + lo), __ldg(seq_start + lo + 1u), position ? __ldg(position + lo) : 0};
     }
     return e;
 }
