@@ -115,13 +115,13 @@ constexpr uint32_t PROMPT_COLUMNS = 256;  // of tensor memory
 
 template <int D>
 struct PromptShape {
-    static constexpr uint32_t TILE = PROMPT_ROWS * D * 2u;  // 128 rows of queries, keys or values
-    static constexpr uint32_t STAGES = D == 128 ? 2 : 4;
+    static constexpr uint32_t TILE = PROMPT_ROWS * D * 2u;  // the queries; 64 keys and 64 values
+    static constexpr uint32_t STAGES = D == 128 ? 2 : 5;
     static constexpr size_t DYN = (1 + STAGES) * TILE + 1024;  // + alignment slack
 };
 
 struct AttnPromptMaps {
-    CUtensorMap q, k, v;  // [token][head][D] 16-bit, box {64, 1, 128}, 128-byte swizzle
+    CUtensorMap q, k, v;  // [token][head][D] 16-bit, box {64, 1, 128 or 64 (k, v)}, 128-byte swizzle
 };
 
 __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint32_t x, uint32_t y,
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 2)
     using L = PromptShape<D>;
     constexpr uint32_t ST = L::STAGES, TMA_WARP = 4, MMA_WARP = 5;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t q_full, kv_full[ST], kv_empty[ST], s_full, p_full[2], o_full;
+    __shared__ __align__(8) uint64_t q_full, kv_full[ST], kv_empty[ST], s_full[2], p_full[2];
     __shared__ uint32_t s_tmem, s_abort;
     __shared__ SeqExtent s_extent;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -239,10 +239,10 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 2)
     }
     if (tid == 0) {
         mbar_init(&q_full, 1);
-        mbar_init(&s_full, 1);
-        mbar_init(&p_full[0], 4);  // one arrival a softmax warp
-        mbar_init(&p_full[1], 4);
-        mbar_init(&o_full, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);  // one arrival a softmax warp
+        }
         for (uint32_t s = 0; s < ST; ++s) {
             mbar_init(&kv_full[s], 1);
             mbar_init(&kv_empty[s], 1);
@@ -270,7 +270,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 2)
     const bool bad = begin < 0 || stop < begin || stop > (int64_t)p.n_tokens;
     if (bad && tid == 0) atomicOr(p.status, WL_DEV_ERR_INDEX);
     const int64_t row0 = ((int64_t)unit - (begin / PROMPT_ROWS + (int64_t)s_extent.seq)) * PROMPT_ROWS;
-    const uint32_t n = !bad && row0 >= 0 && row0 < len ? (uint32_t)(row0 / PROMPT_ROWS) + 1u : 0u;  // steps
+    // steps of 64 keys: to the last that a row of this sequence sees
+    const uint32_t n = !bad && row0 >= 0 && row0 < len ? (uint32_t)(row0 / 64) + (row0 + 64 < len ? 2u : 1u) : 0u;
 
     auto aborted = [&]() { return *(volatile uint32_t *)&s_abort != 0u; };
     auto wait = [&](uint64_t *bar, uint32_t parity) {  // false: the wait ran out, here or elsewhere
@@ -292,22 +293,25 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 2)
         // no rows
     } else if (warp == TMA_WARP) {
         if (lane == 0) {
-            auto load_tile = [&](uint8_t *dst, const CUtensorMap *map, uint32_t y, uint32_t z, uint64_t *bar) {
-                mbar_arrive_expect_tx(bar, L::TILE);
+            // a box of `rows` x 64 elements of each 64 dimensions
+            auto load_tile = [&](uint8_t *dst, const CUtensorMap *map, uint32_t y, uint32_t z, uint32_t rows,
+                                 uint64_t *bar) {
 #pragma unroll
-                for (uint32_t x = 0; x < (uint32_t)D; x += 64) tma_load_3d(dst + x * 256u, map, x, y, z, bar);
+                for (uint32_t x = 0; x < (uint32_t)D; x += 64) tma_load_3d(dst + x * rows * 2u, map, x, y, z, bar);
             };
+            mbar_arrive_expect_tx(&q_full, L::TILE);
+            load_tile(smem, &maps.q, head, (uint32_t)(begin + row0), PROMPT_ROWS, &q_full);
+            // ring entry i: keys of step i and values of step i - 2, used together
             uint32_t it = 0;
-            auto load_kv = [&](const CUtensorMap *map, uint32_t j) {
-                const uint32_t s = it % ST;
-                if (it >= ST && !wait(&kv_empty[s], (it / ST - 1u) & 1u)) return false;
-                load_tile(smem + (1u + s) * L::TILE, map, head / p.group, (uint32_t)begin + j * 128u, &kv_full[s]);
-                ++it;
-                return true;
-            };
-            load_tile(smem, &maps.q, head, (uint32_t)(begin + row0), &q_full);
-            bool ok = true;
-            for (uint32_t j = 0; ok && j < n; ++j) ok = load_kv(&maps.k, j) && load_kv(&maps.v, j);
+            for (; it < n + 2u; ++it) {
+                const uint32_t s = it % ST, h = head / p.group;
+                if (it >= ST && !wait(&kv_empty[s], (it / ST - 1u) & 1u)) break;
+                uint8_t *dst = smem + (1u + s) * L::TILE;
+                mbar_arrive_expect_tx(&kv_full[s], ((it < n) + (it >= 2u)) * (L::TILE / 2u));
+                if (it < n) load_tile(dst, &maps.k, h, (uint32_t)begin + it * 64u, 64u, &kv_full[s]);
+                if (it >= 2u)
+                    load_tile(dst + L::TILE / 2u, &maps.v, h, (uint32_t)begin + (it - 2u) * 64u, 64u, &kv_full[s]);
+            }
             // (bounded) the last copies land before the CTA's shared memory goes
             (void)mbar_wait(&q_full, 0);
             for (uint32_t k = it > ST ? it - ST : 0; k < it; ++k)
@@ -317,48 +321,42 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 2)
         if (lane == 0) {
             const uint32_t base = smem_u32(smem);
             const uint32_t bf = pack16<T>(1.0f, 0.0f) == 0x3F80u;
-            const uint32_t idesc_s = umma_idesc_f16(bf, 0u, 128u), idesc_o = umma_idesc_f16(bf, 1u, D);
-            uint32_t freed = 0;  // ring entries (K0, V0, K1, V1, ...) whose reading is committed
+            const uint32_t idesc_s = umma_idesc_f16(bf, 0u, 64u), idesc_o = umma_idesc_f16(bf, 1u, D);
+            uint32_t freed = 0;  // ring entries whose reading is committed
             auto entry = [&](uint32_t it) { return base + (1u + it % ST) * L::TILE; };
             auto loaded = [&](uint32_t it) { return wait(&kv_full[it % ST], (it / ST) & 1u); };
-            auto free_next = [&]() { umma_commit(&kv_empty[freed++ % ST]); };
-            auto scores = [&](uint32_t it) {  // S = Q K^T
-                const uint32_t k = entry(it);
+            auto scores = [&](uint32_t s) {  // S = Q K^T of step s, into the place of its parity
+                const uint32_t k = entry(s);
 #pragma unroll
-                for (uint32_t i = 0; i < (uint32_t)D / 16; ++i) {
-                    const uint32_t off = (i / 4u) * 16384u + (i % 4u) * 32u;
-                    umma_f16_ss(tmem, umma_desc_sw128(base + off), umma_desc_sw128(k + off), idesc_s, i != 0u);
-                }
-                umma_commit(&s_full);
+                for (uint32_t i = 0; i < (uint32_t)D / 16; ++i)
+                    umma_f16_ss(tmem + (s & 1u) * 64u, umma_desc_sw128(base + (i / 4u) * 16384u + (i % 4u) * 32u),
+                                umma_desc_sw128(k + (i / 4u) * 8192u + (i % 4u) * 32u), idesc_s, i != 0u);
             };
-            bool ok = loaded(0) && wait(&q_full, 0);
-            if (ok) {
+            bool ok = wait(&q_full, 0);
+            for (uint32_t s = 0; ok && s < min(n, 2u); ++s) {
+                if (!(ok = loaded(s))) break;
                 tc_fence_after();
-                scores(0);
-                free_next();
+                scores(s);
+                umma_commit(&s_full[s]);
+                umma_commit(&kv_empty[freed++ % ST]);
+            }
+            if (ok && n == 1u) {  // entry 1 holds nothing
+                ok = loaded(1);
+                if (ok) umma_commit(&kv_empty[freed++ % ST]);
             }
             for (uint32_t j = 0; ok && j < n; ++j) {
-                const uint32_t v = 2u * j + 1u, k = v + 1u;
                 // all that the step needs before its weights, so that nothing comes between
                 // the two products
-                if (!(ok = loaded(v) && (j + 1 >= n || loaded(k)))) break;
+                if (!(ok = loaded(j + 2u) && wait(&p_full[j & 1u], (j >> 1) & 1u))) break;
+                tc_fence_after();
+                const uint32_t v = entry(j + 2u) + L::TILE / 2u;
 #pragma unroll
-                for (uint32_t half = 0; half < 2; ++half) {  // O += W V, each half when its weights are there
-                    ok = ok && wait(&p_full[half], j & 1u);
-                    if (!ok) break;
-                    tc_fence_after();
-#pragma unroll
-                    for (uint32_t i = 4 * half; i < 4 * half + 4; ++i)
-                        umma_f16_ts(tmem + 128u, tmem + i * 8u, umma_desc_mn_sw128(entry(v) + i * 2048u, 16384u),
-                                    idesc_o, j != 0u || i != 0u);
-                }
-                if (!ok) break;
-                if (j + 1 < n)
-                    scores(k);
-                else
-                    umma_commit(&o_full);
-                free_next();
-                if (j + 1 < n) free_next();
+                for (uint32_t i = 0; i < 4; ++i)  // O += W V
+                    umma_f16_ts(tmem + 128u, tmem + (j & 1u) * 64u + i * 8u, umma_desc_mn_sw128(v + i * 2048u, 8192u),
+                                idesc_o, j != 0u || i != 0u);
+                if (j + 2u < n) scores(j + 2u);
+                umma_commit(&s_full[j & 1u]);  // of step j + 2, and that the product of step j is done
+                umma_commit(&kv_empty[freed++ % ST]);
             }
             // (bounded) every committed product is done before tensor memory goes
             for (uint32_t k = freed > ST ? freed - ST : 0; k < freed; ++k)
@@ -366,55 +364,48 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 2)
         }
     } else {
         const uint32_t r = tid;  // row in the tile
-        const uint32_t ts = tmem + ((warp * 32u) << 16), to = ts + 128u;
+        const uint32_t lanes = tmem + ((warp * 32u) << 16), to = lanes + 128u;
         const float sc = p.scale * 1.4426950408889634f;
         float m = 0.0f, l = 0.0f;  // m: the maximum in use, in log2 units
         bool ok = true, fine = true;
-        // one step; DIAG: the last, where row r sees keys 0 .. r of the 128 (a code path of
-        // its own, so that the others carry no masks)
-        auto step = [&](uint32_t j, auto last) {
+        // one step; DIAG: of the last two, where row r sees keys 0 .. `seen` of the 64 (a code
+        // path of its own, so that the others carry no masks)
+        auto step = [&](uint32_t j, int seen, auto last) {
             constexpr bool DIAG = decltype(last)::value;
-            // the scores 32 at a time, the second half first: the first stays in registers
-            // for the weights, the second is read again (all 128 in registers would leave
-            // too few for the exponentials to overlap)
-            uint32_t s[3][32];
+            const uint32_t ts = lanes + (j & 1u) * 64u;
+            uint32_t s[64];
+            tmem_ld32(ts, s);
+            tmem_ld32(ts + 32u, s + 32);
+            tmem_wait_ld();
+            auto score = [&](int i) { return __uint_as_float(s[i]); };
             float hi[4], lo[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) hi[q] = -INFINITY, lo[q] = INFINITY;
+            if constexpr (DIAG) {
 #pragma unroll
-            for (int half = 1; half >= 0; --half) {
-                tmem_ld32(ts + 64u * half, s[0]);
-                tmem_ld32(ts + 64u * half + 32u, s[1]);
-                tmem_wait_ld();
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    auto score = [&](int i) { return __uint_as_float(s[c][i]); };
-                    if constexpr (DIAG) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            if ((uint32_t)(64 * half + 32 * c + i) <= r) {
-                                hi[i & 3] = max3_nan(hi[i & 3], score(i), score(i));
-                                lo[i & 3] = min3_nan(lo[i & 3], score(i), score(i));
-                            }
-                        }
-                    } else if (sc >= 0.0f) {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2)
-                            hi[(i / 2) & 3] = max3_nan(hi[(i / 2) & 3], score(i), score(i + 1));
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2)
-                            lo[(i / 2) & 3] = min3_nan(lo[(i / 2) & 3], score(i), score(i + 1));
+                for (int i = 0; i < 64; ++i) {
+                    if (i <= seen) {
+                        hi[i & 3] = max3_nan(hi[i & 3], score(i), score(i));
+                        lo[i & 3] = min3_nan(lo[i & 3], score(i), score(i));
                     }
                 }
+            } else if (sc >= 0.0f) {
+#pragma unroll
+                for (int i = 0; i < 64; i += 2) hi[(i / 2) & 3] = max3_nan(hi[(i / 2) & 3], score(i), score(i + 1));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 64; i += 2) lo[(i / 2) & 3] = min3_nan(lo[(i / 2) & 3], score(i), score(i + 1));
             }
             float top = sc >= 0.0f ? max3_nan(max3_nan(hi[0], hi[1], hi[2]), hi[3], hi[3])
                                    : min3_nan(min3_nan(lo[0], lo[1], lo[2]), lo[3], lo[3]);
-            top *= sc;
+            top = DIAG && seen < 0 ? -INFINITY : top * sc;
             fine = fine && top < INFINITY;  // NaN or infinite scores: the row is computed again
             if (j == 0) {
                 m = top;
             } else if (__any_sync(0xffffffffu, top > m + 8.0f)) {
+                // the product of step j - 1 is done when the scores of step j + 1 are there
+                if (!wait_all(&s_full[(j + 1u) & 1u], ((j + 1u) >> 1) & 1u)) return false;
+                tc_fence_after();
                 const float mn = fmaxf(m, top);
                 const float f = mn == -INFINITY ? 1.0f : ex2_approx(m - mn);
                 l *= f;
@@ -431,51 +422,36 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 2)
             }
             const float base = 6.0f - (m == -INFINITY ? 0.0f : m);
             float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-            auto weigh = [&](uint32_t (&v)[32], uint32_t (&w)[32], int chunk) {  // 32 scores to 16 pairs of weights
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float2 x = f2_fma_rn(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])),
-                                               make_float2(sc, sc), make_float2(base, base));
-                    float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-                    if constexpr (DIAG) {
-                        e.x = (uint32_t)(32 * chunk + i) <= r ? e.x : 0.0f;
-                        e.y = (uint32_t)(32 * chunk + i + 1) <= r ? e.y : 0.0f;
-                    }
-                    sum[(i / 2) & 1] = f2_add_rn(sum[(i / 2) & 1], e);
-                    w[16 * (chunk & 1) + i / 2] = pack16<T>(e.x, e.y);
+            for (int i = 0; i < 64; i += 2) {
+                const float2 x = f2_fma_rn(make_float2(score(i), score(i + 1)), make_float2(sc, sc),
+                                           make_float2(base, base));
+                float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                if constexpr (DIAG) {
+                    e.x = i <= seen ? e.x : 0.0f;
+                    e.y = i + 1 <= seen ? e.y : 0.0f;
                 }
-            };
-            auto hand_over = [&](const uint32_t (&w)[32], int half) {
-                tmem_st32(ts + 32u * half, w);
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[half]);
-            };
-            uint32_t w[32];
-            tmem_ld32(ts + 64u, s[2]);
-            weigh(s[0], w, 0);
-            weigh(s[1], w, 1);
-            tmem_wait_ld();
-            tmem_ld32(ts + 96u, s[0]);
-            hand_over(w, 0);
-            weigh(s[2], w, 2);
-            tmem_wait_ld();
-            weigh(s[0], w, 3);
-            hand_over(w, 1);
+                sum[(i / 2) & 1] = f2_add_rn(sum[(i / 2) & 1], e);
+                s[i / 2] = pack16<T>(e.x, e.y);
+            }
+            tmem_st32(ts, s);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[j & 1u]);
             sum[0] = f2_add_rn(sum[0], sum[1]);
             l += sum[0].x + sum[0].y;
+            return true;
         };
-        for (uint32_t j = 0; j < n; ++j) {
-            ok = wait_all(&s_full, j & 1u);
-            if (!ok) break;
+        const uint32_t plain = (uint32_t)(row0 / 64);  // steps without a mask
+        for (uint32_t j = 0; ok && j < n; ++j) {
+            if (!(ok = wait_all(&s_full[j & 1u], (j >> 1) & 1u))) break;
             tc_fence_after();
-            if (j + 1 < n)
-                step(j, std::false_type());
-            else
-                step(j, std::true_type());
+            ok = j < plain ? step(j, 63, std::false_type()) : step(j, (int)r - 64 * (int)(j - plain), std::true_type());
         }
-        if (ok && wait_all(&o_full, 0)) {
+        // the last two products
+        if (ok && n > 1u) ok = wait_all(&s_full[n & 1u], (n >> 1) & 1u);
+        if (ok && wait_all(&s_full[(n + 1u) & 1u], ((n + 1u) >> 1) & 1u)) {
             tc_fence_after();
             const int64_t row = begin + row0 + r;
             const bool mine = row0 + r < len;

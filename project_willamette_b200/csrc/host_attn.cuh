@@ -115,13 +115,13 @@ int launch_kv_append(KvAppendParams &p, cudaStream_t s) {
     return launch_kv_append_as<T, 4, 256, 1, true>(p, s);
 }
 
-// Tensor map of [n_tokens][heads][D] 16-bit rows `stride` elements apart: 128 tokens
+// Tensor map of [n_tokens][heads][D] 16-bit rows `stride` elements apart: box_rows tokens
 // x 64 elements of one head, 128-byte swizzle, zeros behind the last token.
 int encode_heads(EncodeTiledFn enc, CUtensorMap *map, const void *base, uint32_t n_tokens,
-                 uint32_t heads, uint32_t D, uint64_t stride) {
+                 uint32_t heads, uint32_t D, uint64_t stride, uint32_t box_rows) {
     const cuuint64_t dims[3] = {D, heads, n_tokens};
     const cuuint64_t strides[2] = {D * 2ull, stride * 2ull};
-    const cuuint32_t box[3] = {64, 1, 128};
+    const cuuint32_t box[3] = {64, 1, box_rows};
     const cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void *>(base), dims, strides, box,
                      estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -136,9 +136,9 @@ int launch_attn_prompt(const AttnPromptParams &p, uint32_t D, cudaStream_t s) {
     int rc = get_encode_tiled(&enc);
     if (rc) return rc;
     AttnPromptMaps maps;
-    if ((rc = encode_heads(enc, &maps.q, p.q, p.n_tokens, p.n_kv * p.group, D, p.q_stride)) ||
-        (rc = encode_heads(enc, &maps.k, p.k, p.n_tokens, p.n_kv, D, p.k_stride)) ||
-        (rc = encode_heads(enc, &maps.v, p.v, p.n_tokens, p.n_kv, D, p.v_stride)))
+    if ((rc = encode_heads(enc, &maps.q, p.q, p.n_tokens, p.n_kv * p.group, D, p.q_stride, PROMPT_ROWS)) ||
+        (rc = encode_heads(enc, &maps.k, p.k, p.n_tokens, p.n_kv, D, p.k_stride, 64)) ||
+        (rc = encode_heads(enc, &maps.v, p.v, p.n_tokens, p.n_kv, D, p.v_stride, 64)))
         return rc;
     // sequence s owns the units [seq_start[s] / 128 + s, ...), at least as many as it needs
     const uint64_t ctas = ((uint64_t)p.n_tokens / PROMPT_ROWS + p.n_seqs) * p.n_kv * p.group;
