@@ -7,6 +7,35 @@
 //   out = (sum_i exp(z_i - m) * vs[P(i)] * vq_i) / (sum_i exp(z_i - m)),
 // zeros where n = 0.  Keys at and behind n take no part: their codes are
 // finite whatever they hold, and a page without a key below n is not read.
+//
+// Arithmetic.  A warp takes 32 keys at a time on m16n8k16 tiles (f16 x f16 -> f32).
+// A code is exact in f16 (its byte under the exponent of 1024, minus 1152).  q, scaled by
+// a power of two, and the weights exp(z - m) * 2^14 are each split into two f16 numbers,
+// hi in tile rows 0-7 and lo in rows 8-15, so that a tile's 16 rows serve 8 query heads
+// with 22 bits and the f32 sums of hi and lo land in the same lane.  exp is 2^x by
+// the hardware's approximation (2^-22) of scores in log2 units.  The values' scale
+// enters the weights relative to the largest scale so far, as the scores enter
+// relative to their maximum.  Groups of more than 8 heads take several passes.
+//
+// Work.  Units of 128 keys of all (sequence, KV head, pass) items, plus one for each
+// item's beginning, are cut into equal contiguous shares, one for each of three
+// CTAs an SM, from the lengths on the device: no share waits for a long sequence and a
+// captured graph stays balanced as lengths grow.  Every warp copies its tiles (8 KB of K
+// and V at D = 128) by TMA into a ring of its own, across its segments.  An item cut
+// between CTAs is joined by the last CTA to arrive, in CTA order, so results repeat.
+//
+// Bound by HBM: 2 bytes a key, head and dimension, 4 G flops each.  In the steady state an
+// SM moves 96 KB in 4300 cycles, 6.4 TB/s over the chip (a plain copy reaches 6.55); what is
+// left is a call's beginning and end (about 10 us, all of a small call).  Measured
+// (median call in a captured chain): 64 sequences to 8192 keys, 5 KV heads of 128, 64.7 us
+// = 4.49 TB/s (0.69 of the copy); 4 sequences to 100,000 keys, 4 KV heads, 74.9 us = 4.63
+// TB/s; 32 sequences to 1024 keys, 3 KV heads of 64, 10.1 us; one of 640 keys, 5 heads of
+// 128, 10.7 us.  Steps on the way at 64 x 8192: one CTA a (query head, sequence) on the
+// CUDA cores 6169 us; tiles from registers 160; TMA rings 95; vector query loads and
+// joins by whole warps 75; three CTAs an SM instead of two 71; beginnings counted in the
+// shares 64.7.  Not kept: scores as exact s8 products of three query digits
+// (m16n8k32; 71.2: the conversions it saves are not what bounds it, and it spills), the
+// joining as a kernel of its own (89.8: a chain of calls then waits twice).
 #pragma once
 
 #include <cuda.h>
@@ -32,11 +61,6 @@ struct AttnDecodeParams {
     uint32_t *status;
 };
 
-__device__ __forceinline__ float load_typed(const void *base, uint32_t type, size_t at) {
-    if (type == 0u) return static_cast<const float *>(base)[at];
-    if (type == 1u) return __half2float(static_cast<const __half *>(base)[at]);
-    return __bfloat162float(static_cast<const __nv_bfloat16 *>(base)[at]);
-}
 __device__ __forceinline__ void store_typed(void *base, uint32_t type, size_t at, float x) {
     if (type == 0u)
         static_cast<float *>(base)[at] = x;

@@ -84,31 +84,43 @@ __device__ __forceinline__ void prompt_row(const AttnPromptParams &p, int64_t be
 }
 
 // ------------------------------------------------------------------ tensor cores
-// A CTA takes 128 rows of one head and goes through the keys 128 at a time; two CTAs
-// share an SM, so that one's softmax runs beside the other's products.  Tensor memory
-// (256 columns a CTA): scores (128 f32 columns; the weights overwrite them as 16-bit
-// pairs) and output (D f32 columns).
+// A CTA takes 128 rows of one head and goes through the keys 64 at a time; two CTAs share
+// an SM, so that one's softmax runs beside the other's products.  Tensor memory (256
+// columns a CTA): the scores of two steps (64 f32 columns each; the weights overwrite
+// them as 16-bit pairs) and the output (D f32 columns).
 //   warps 0-3  softmax, one thread a row: scores to registers, row maximum, weights
-//              2^(z - m + 6) back as 16-bit, by halves; the output is rescaled only when
-//              the maximum has risen by more than 2^8 over the one in use (weights then
-//              stay below 2^14);
-//   warp 4     TMA: queries, then keys and values through a ring;
+//              2^(z - m + 6) back as 16-bit; the output is rescaled only when the
+//              maximum has risen by more than 2^8 over the one in use (weights then stay
+//              below 2^14);
+//   warp 4     TMA: queries, then ring entries of the keys of step i and the values of
+//              step i - 2, which are used together;
 //   warp 5     MMA (one thread): weights x values of step j, then queries x keys of step
-//              j + 1, with nothing between them (a commit there cost a tenth of the time).
-// The commit on the scores of step j + 1 covers the product into the output before it,
-// so who reads those scores may also rescale the output.
+//              j + 2 into the scores' place that step j leaves, with nothing between
+//              them (a commit there cost a tenth of the time).  A softmax warp finds its
+//              next scores ready when it hands over its weights.
+// The commit of both says that the scores of step j + 2 are there and that the product
+// of step j is in the output.
 // The masked part of a product is 0 x v, which is NaN where v is not finite: a row whose
 // scores or output are not finite is computed again by prompt_row, which does not read
 // what the mask leaves out.
-// What bounds it at D = 128: an SM's step of 128 x 128 takes 1090 cycles of products (64
-// to 70 an MMA, whose N = 64 costs as much as N = 128) and 1030 of exponentials (16 a
-// cycle), but a softmax warp needs 2200 from its scores to its last weights, and the next
-// scores are another 1000 away; two CTAs cover each other's waits to about 1850 a step.
-// Measured beside it: two tiles in one CTA of 10 warps (1 x 512 tokens of 20 heads 16.6
-// against 14.3 us, 32 x 256 72 against 62, 2 x 4096 198 against 187); 64-key steps with
-// two score buffers (763 against 600 us at 2 x 8k); weights through shared memory, so
-// that the next scores come beside the softmax (589 against 581); a part of the
-// exponentials by polynomial (4 to 20 % slower: the issue slots are what is short).
+//
+// What bounds it: at D = 128 an SM's 128 keys of a tile take 1650 cycles of products (an
+// MMA of M = 128 takes 64 to 70 cycles for N = 64 as for N = 128) and 1030 of exponentials
+// (16 a cycle and SM), a softmax warp 2400 from scores to weights, and two CTAs overlap
+// these to about 1750; long prompts also run into the power limit (2 x 8192: 544 to 600 us
+// by the run).  At D = 64 the softmax alone bounds it.  Short prompts pay each CTA's
+// beginning and end, 6000 cycles.  Measured (median call in a captured chain): 2 prompts to
+// 8192 tokens, 20 / 5 heads of 128, bf16, 544 us = 1106 TFLOP/s of the causal half (0.66
+// of cuBLAS's dense rate); 2048 tokens f16 36.1 us; 32 packed prompts to 1024 tokens, 9 / 3
+// heads of 64, 53.6 us; 77 tokens 6.0 us.
+// Steps on the way, at 2 x 8192: rows on the CUDA cores 100.8 ms; two tiles a CTA of 10
+// warps, 128-key steps 654 us; the masked last step a code path of its own (its 128
+// predicates had been kept in registers through every step) 581; one tile a CTA, two CTAs
+// an SM 624 (32 packed prompts 77 -> 66); 64-key steps with two score buffers 547 (54).
+// Not kept: weights through shared memory instead of tensor memory (589 against 581),
+// a part of the exponentials by polynomial (1 to 20 % slower at each stage: the issue
+// slots are what is short), MMAs issued by predicate from a convergent warp (45 against
+// 41 us at 2048 tokens).
 constexpr int PROMPT_THREADS = 192;
 constexpr uint32_t PROMPT_ROWS = 128;
 constexpr uint32_t PROMPT_COLUMNS = 256;  // of tensor memory

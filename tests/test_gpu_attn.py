@@ -96,6 +96,25 @@ def test_append_prompts_and_steps(page, dim, kv, group, n_rot, pairs, dtype, out
                rope, n_rot, pairs, heads, out, copies=False)
 
 
+@pytest.mark.parametrize("dim,dtype", [(64, F32), (128, BF16), (128, F32)])
+def test_append_one_prompt_among_many_steps(dim, dtype):
+    """A call made for single tokens that brings one long prompt as well: its pages hold more rows than
+    the threads that such a call gets keep in registers."""
+    g = gen(4)
+    page, kv, group, n_rot = 128, 3, 2, 64
+    lengths = [1] * 60 + [150] + [1] * 130
+    position = [int(x) for x in np.random.default_rng(1).integers(0, 2 * page, len(lengths))]
+    need = [-(-(a + b) // page) for a, b in zip(lengths, position)]
+    order = torch.randperm(sum(need), generator=gen(2), device="cuda").tolist()
+    table = [[order.pop() for _ in range(m)] + [0] * (max(need) - m) for m in need]
+    c = Cache(sum(need), page, kv, dim, fill=3)
+    c.ks.uniform_(0.001, 0.05, generator=g)
+    c.vs.uniform_(0.001, 0.05, generator=g)
+    T = sum(lengths)
+    q, k, v = (randn(g, T, n * dim, dtype=dtype) for n in (kv * group, kv, kv))
+    run_append(c, q, k, v, lengths, position, table, rope_table(3 * page + 200, n_rot), n_rot, 0, kv * group, F16)
+
+
 def test_append_token_by_token_stays_within_a_step():
     """A page filled one token at a time with ever larger values: every value within one step of the
     page's last scale, and within half a step where the page was written by one call."""
@@ -271,6 +290,53 @@ def test_decode_strides_and_rows_beyond_the_lengths():
     once = out.clone()
     decode(c, q, i32(lengths), t, heads, 0.2, out=out[:, 16:16 + heads * dim])
     assert torch.equal(once, out)
+
+
+def test_decode_one_workspace_for_every_shape():
+    """Calls of other head sizes, batches and groups one after another over one workspace."""
+    g = gen(16)
+    ws = workspace(1, 1, Cache(1, 16, 1, 128))
+    for page, dim, kv, group, lengths in [(16, 64, 2, 3, [5000, 3]), (64, 128, 5, 4, [700] * 30), (32, 128, 1, 9, [20000]),
+                                          (128, 64, 3, 3, [1]), (16, 128, 2, 2, [0, 0]), (64, 64, 1, 1, [333] * 5)]:
+        total, table = tables(g, lengths, page)
+        c = filled(g, total, page, kv, dim)
+        q = randn(g, len(lengths), kv * group * dim)
+        t = i32(table)
+        ref, tol = decode_ref(c, q, lengths, t, kv * group, 0.1)
+        within(decode(c, q, i32(lengths), t, kv * group, 0.1, ws=ws), ref, tol)
+    assert (ws[:1024] == 0).all()  # the counters
+
+
+def test_calls_on_two_streams_at_once():
+    """Decode over two caches, each with its own workspace, and a prompt, all in flight together."""
+    g = gen(17)
+    work = []
+    for page, dim, kv, group, lengths in [(64, 128, 5, 4, [9000, 500, 20000]), (32, 64, 3, 3, [4000] * 20)]:
+        total, table = tables(g, lengths, page)
+        c = filled(g, total, page, kv, dim)
+        q = randn(g, len(lengths), kv * group * dim)
+        t = i32(table)
+        work.append((c, q, i32(lengths), t, kv * group, workspace(len(lengths), kv * group, c),
+                     decode_ref(c, q, lengths, t, kv * group, 0.1)))
+    lengths = [700, 900]
+    q, k, v = (randn(g, sum(lengths), n * 64, dtype=F16) for n in (4, 2, 2))
+    pref, ptol = prompt_ref(q, k, v, lengths, 4, 2, 64, 0.1)
+    start = starts(lengths)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = [[], [], []]
+    for _ in range(5):
+        for i, (c, x, n, t, heads, ws, _) in enumerate(work):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(decode(c, x, n, t, heads, 0.1, ws=ws))
+        with torch.cuda.stream(streams[2]):
+            outs[2].append(prompt(q, k, v, start, 4, 2, 64, 0.1))
+    torch.cuda.synchronize()
+    for i, w in enumerate(work):
+        for o in outs[i]:
+            within(o, *w[6])
+    for o in outs[2]:
+        within(o, pref, ptol)
 
 
 def test_decode_not_finite():
@@ -473,6 +539,31 @@ def test_prompt_masked_rows_have_no_effect(dim, dtype, bad):
             others = [i for i in range(dim) if i != 3]
             r, a = (y[sees].view(-1, heads, dim)[:, 2:][..., others] for y in (ref, tol))
             within(mine[..., others], r, a)
+
+
+def test_prompt_captured_and_replayed():
+    """A captured call replayed with other values and other borders between the sequences."""
+    g = gen(26)
+    heads, kv, dim, T = 4, 2, 128, 600
+    q, k, v = (torch.empty(T, n * dim, dtype=BF16, device="cuda") for n in (heads, kv, kv))
+    start = i32([0, 100, 100, 600])
+    out = torch.empty(T, heads * dim, dtype=BF16, device="cuda")
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        prompt(q, k, v, start, heads, kv, dim, 0.1, out=out)
+    for lengths in ([100, 0, 500], [1, 598, 1], [0, 300, 129]):
+        for x in (q, k, v):
+            x.copy_(randn(g, *x.shape))
+        start.copy_(starts(lengths))
+        out.fill_(3)
+        graph.replay()
+        torch.cuda.synchronize()
+        used = sum(lengths)
+        ref, tol = prompt_ref(q, k, v, lengths, heads, kv, dim, 0.1)
+        within(out[:used], ref, tol)
+        assert (out[used:] == 3).all()
+    assert status() == 0
 
 
 def test_prompt_bad_extents_are_left_out_and_reported():
