@@ -428,7 +428,8 @@ int wl_dev_attn_decode_i8(const wl_kv_pages_i8 *cache, const wl_attn_decode *arg
 
 /* Causal attention within packed prompts: row i of sequence s (rows
  * seq_start[s] .. seq_start[s + 1] of q, k, v) attends to rows 0 .. i of the
- * same sequence.  What masked rows hold, NaN included, has no effect.  Rows
+ * same sequence.  Sequences are begun in the caller's order: long prompts are
+ * best put first.  What masked rows hold, NaN included, has no effect.  Rows
  * of out that no sequence owns are left as they were.  q, k and v are all
  * WL_GGML_F16 or all WL_GGML_BF16; out is that type or WL_GGML_F32.  Scores,
  * softmax and sums in f32; the weights enter the product with v in the

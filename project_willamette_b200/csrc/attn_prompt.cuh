@@ -111,12 +111,13 @@ __device__ __forceinline__ void prompt_row(const AttnPromptParams &p, int64_t be
 // by the run).  At D = 64 the softmax alone bounds it.  Short prompts pay each CTA's
 // beginning and end, 6000 cycles.  Measured (median call in a captured chain): 2 prompts to
 // 8192 tokens, 20 / 5 heads of 128, bf16, 544 us = 1106 TFLOP/s of the causal half (0.66
-// of cuBLAS's dense rate); 2048 tokens f16 36.1 us; 32 packed prompts to 1024 tokens, 9 / 3
-// heads of 64, 53.6 us; 77 tokens 6.0 us.
+// of cuBLAS's dense rate); 2048 tokens f16 35.8 us; 32 packed prompts to 1024 tokens, 9 / 3
+// heads of 64, 49.4 us; 77 tokens 6.0 us.
 // Steps on the way, at 2 x 8192: rows on the CUDA cores 100.8 ms; two tiles a CTA of 10
 // warps, 128-key steps 654 us; the masked last step a code path of its own (its 128
 // predicates had been kept in registers through every step) 581; one tile a CTA, two CTAs
-// an SM 624 (32 packed prompts 77 -> 66); 64-key steps with two score buffers 547 (54).
+// an SM 624 (32 packed prompts 77 -> 66); 64-key steps with two score buffers 547 (54);
+// sequences in order, not from the last, (49).
 // Not kept: weights through shared memory instead of tensor memory (589 against 581),
 // a part of the exponentials by polynomial (1 to 20 % slower at each stage: the issue
 // slots are what is short), MMAs issued by predicate from a convergent warp (45 against
@@ -239,9 +240,9 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 2)
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                 ~(uintptr_t)1023);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
-    // longest rows first: units in descending order, heads side by side
-    const uint32_t heads = p.n_kv * p.group, head = blockIdx.x % heads;
-    const uint32_t unit = (gridDim.x - 1u - blockIdx.x) / heads;
+    // sequences in the caller's order, the last rows of each (the longest) first, heads side
+    // by side: a tail of long tiles at the end of the grid cost 4 of 54 us at 32 prompts
+    const uint32_t heads = p.n_kv * p.group, head = blockIdx.x % heads, unit = blockIdx.x / heads;
 
     if (warp == MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -281,9 +282,11 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 2)
     const int64_t begin = s_extent.begin, stop = s_extent.end, len = stop - begin;
     const bool bad = begin < 0 || stop < begin || stop > (int64_t)p.n_tokens;
     if (bad && tid == 0) atomicOr(p.status, WL_DEV_ERR_INDEX);
-    const int64_t row0 = ((int64_t)unit - (begin / PROMPT_ROWS + (int64_t)s_extent.seq)) * PROMPT_ROWS;
+    const int64_t tiles = (len + PROMPT_ROWS - 1) / PROMPT_ROWS;
+    const int64_t place = (int64_t)unit - (begin / PROMPT_ROWS + (int64_t)s_extent.seq);
+    const int64_t row0 = (tiles - 1 - place) * PROMPT_ROWS;
     // steps of 64 keys: to the last that a row of this sequence sees
-    const uint32_t n = !bad && row0 >= 0 && row0 < len ? (uint32_t)(row0 / 64) + (row0 + 64 < len ? 2u : 1u) : 0u;
+    const uint32_t n = !bad && place >= 0 && place < tiles ? (uint32_t)(row0 / 64) + (row0 + 64 < len ? 2u : 1u) : 0u;
 
     auto aborted = [&]() { return *(volatile uint32_t *)&s_abort != 0u; };
     auto wait = [&](uint64_t *bar, uint32_t parity) {  // false: the wait ran out, here or elsewhere
