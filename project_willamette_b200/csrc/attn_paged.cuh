@@ -18,24 +18,28 @@
 // relative to their maximum.  Groups of more than 8 heads take several passes.
 //
 // Work.  Units of 128 keys of all (sequence, KV head, pass) items, plus one for each
-// item's beginning, are cut into equal contiguous shares, one for each of three
-// CTAs an SM, from the lengths on the device: no share waits for a long sequence and a
-// captured graph stays balanced as lengths grow.  Every warp copies its tiles (8 KB of K
-// and V at D = 128) by TMA into a ring of its own, across its segments.  An item cut
-// between CTAs is joined by the last CTA to arrive, in CTA order, so results repeat.
+// item's beginning, are cut into equal contiguous shares, one for each of two CTAs an SM
+// (fewer where the page table has no room for as many places), from the lengths on the
+// device: no share waits for a long sequence and a captured graph stays balanced as
+// lengths grow.  Every warp copies its tiles (8 KB of K and V at D = 128) by TMA into a
+// ring of its own, across its segments.  An item cut between CTAs is joined by the last
+// CTA to arrive, in CTA order, so results repeat.
 //
-// Bound by HBM: 2 bytes a key, head and dimension, 4 G flops each.  In the steady state an
-// SM moves 96 KB in 4300 cycles, 6.4 TB/s over the chip (a plain copy reaches 6.55); what is
-// left is a call's beginning and end (about 10 us, all of a small call).  Measured
-// (median call in a captured chain): 64 sequences to 8192 keys, 5 KV heads of 128, 64.7 us
-// = 4.49 TB/s (0.69 of the copy); 4 sequences to 100,000 keys, 4 KV heads, 74.9 us = 4.63
-// TB/s; 32 sequences to 1024 keys, 3 KV heads of 64, 10.1 us; one of 640 keys, 5 heads of
-// 128, 10.7 us.  Steps on the way at 64 x 8192: one CTA a (query head, sequence) on the
-// CUDA cores 6169 us; tiles from registers 160; TMA rings 95; vector query loads and
-// joins by whole warps 75; three CTAs an SM instead of two 71; beginnings counted in the
-// shares 64.7.  Not kept: scores as exact s8 products of three query digits
-// (m16n8k32; 71.2: the conversions it saves are not what bounds it, and it spills), the
-// joining as a kernel of its own (89.8: a chain of calls then waits twice).
+// Bound by HBM: 2 bytes a key, head and dimension, 4 G flops each; in the steady state the
+// copies run near a plain copy's rate (6.55 TB/s), and what is left is a call's beginning
+// and end (about 9 us, all of a small call).  Measured (median call in a captured chain):
+// 64 sequences to 8192 keys, 5 KV heads of 128, 65.9 us = 4.41 TB/s (0.67 of the copy); 4
+// sequences to 100,000 keys, 4 KV heads, 74.2 us = 4.67 TB/s; 32 sequences to 1024 keys, 3
+// KV heads of 64, 9.8 us; one of 640 keys, 5 heads of 128, 9.0 us.  Three CTAs an SM at
+// 168 registers (spilling) instead of two at 212: 64.8, 75.2, 10.1 and 10.7; rings of 24
+// KB a warp instead of 16 at D = 128: 67.6, 76.9; rings of 16 KB instead of 24 at D = 64:
+// 10.3 for 9.8; CTAs without a place not launched: 9.25 to 9.0.  Steps on the way at 64 x
+// 8192: one CTA a (query head, sequence) on the CUDA cores 6169 us; tiles from registers
+// 160; TMA rings 95; vector query loads and joins by whole warps 75; three CTAs an SM 71;
+// beginnings counted in the shares 64.7; two CTAs again, as above.  Not kept: scores as
+// exact s8 products of three query digits (m16n8k32; 71.2: the conversions it saves are
+// not what bounds it, and it spills), the joining as a kernel of its own (89.8: a chain of
+// calls then waits twice).
 #pragma once
 
 #include <cuda.h>
@@ -74,7 +78,7 @@ constexpr int PAGED_THREADS = 128;
 constexpr int PAGED_WARPS = PAGED_THREADS / 32;
 constexpr int PAGED_TILE = 32;                           // keys of a warp's step
 constexpr int PAGED_UNIT = PAGED_TILE * PAGED_WARPS;     // keys of a CTA's step: the unit of work
-constexpr int PAGED_CTAS_PER_SM = 3;
+constexpr int PAGED_CTAS_PER_SM = 2;
 constexpr int PAGED_MAX_CTAS = 148 * PAGED_CTAS_PER_SM;
 constexpr int PAGED_JOIN = 16;                          // parts of a row read at once when joined
 constexpr int PAGED_ROWS = 8;                            // query heads of one pass over the keys
@@ -122,7 +126,7 @@ __device__ __forceinline__ void split_f16(float v0, float v1, uint32_t &hi, uint
 
 template <int D>
 struct PagedSmem {
-    static constexpr uint32_t STAGES = D == 128 ? 2 : 4;
+    static constexpr uint32_t STAGES = D == 128 ? 2 : 6;
     static constexpr uint32_t HALF = PAGED_TILE * D;   // a tile's keys; its values follow
     static constexpr uint32_t STAGE = 2u * HALF;
     static constexpr uint32_t WARP = STAGES * STAGE;
@@ -467,7 +471,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
         if (more) {
             // the pass's query rows: row g as f16 parts hi (tile row g) and lo (row
             // g + 8) of q * 2^shift, its largest |q| brought to [2^13, 2^14).  Kept in
-            // shared memory: in registers they would take the room of a third CTA's
+            // shared memory: in registers they measured the same (66.5 us for 65.9)
             const PagedSegment &sg = s_sg[turn];
             if (joining) begin_segment(sg);
             uint4 raw[D / 16];

@@ -294,8 +294,12 @@ int wl_dev_attn_decode_i8(const wl_kv_pages_i8 *cache, const wl_attn_decode *a, 
     p.max_pages = a->max_pages;
     p.scale = a->scale;
     p.workspace = a->workspace;
-    const uint32_t ctas = std::min<uint32_t>((uint32_t)sm_count_for_launch() * PAGED_CTAS_PER_SM,
-                                             PAGED_MAX_CTAS);
+    // no more CTAs than the longest lengths that the table allows have places of work
+    const uint32_t passes = (p.group + PAGED_ROWS - 1) / PAGED_ROWS;
+    const uint64_t units = (((uint64_t)a->max_pages << p.page_shift) + PAGED_UNIT - 1) / PAGED_UNIT;
+    const uint32_t ctas = (uint32_t)std::min<uint64_t>(
+        std::min<uint32_t>((uint32_t)sm_count_for_launch() * PAGED_CTAS_PER_SM, PAGED_MAX_CTAS),
+        (units + 1) * KV * passes * a->n_seqs);
     auto kernel = cache->page_size == 16
                       ? (D == 64 ? attn_decode_i8_kernel<64, true> : attn_decode_i8_kernel<128, true>)
                       : (D == 64 ? attn_decode_i8_kernel<64, false> : attn_decode_i8_kernel<128, false>);
