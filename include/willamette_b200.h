@@ -373,9 +373,10 @@ typedef struct wl_kv_pages_i8 {
  * new values fit and is doubled as often as they need otherwise; the codes in
  * front of the new ones are then rounded again to the doubled steps.  So a
  * value's code is off by at most half a step of the scale that it was written
- * with, and by less than one step of the page's last scale.  Rows behind the
- * new ones are left as they are.  NaN or infinity among a page's new values
- * makes its scale NaN.
+ * with, and by less than one step of the page's last scale.  A page that was
+ * filled by other means may have a negative scale: it keeps its sign and grows
+ * by its size.  Rows behind the new ones are left as they are.  NaN or infinity
+ * among a page's new values makes its scale NaN.
  * rope: [rope_len][n_rot / 2] pairs (cos, sin), one row per position (any
  * frequency scaling is the table's); elements from n_rot on are not rotated;
  * n_rot 0: none (rope may be NULL).  Products and sums are rounded to f32 one

@@ -8,9 +8,9 @@
 //   the page's scale (one for each page and KV head, of K and of V apart):
 //     need = (largest |x| of the call's new rows in the page) / 127
 //     s    = need                       where the call begins the page
-//          = s_old                      where need <= s_old
+//          = s_old                      where need <= |s_old|
 //          = need                       where s_old = 0
-//          = s_old * 2^k                else, k the smallest with s >= need;
+//          = s_old * 2^k                else, k the smallest with |s| >= need;
 //     the codes in front of the new ones become rint(code / 2^k);
 //   codes  rint(x / s) in [-127, 127], 0 where s is 0 or NaN.
 // A scale grows by whole doublings because the codes that are there already
@@ -44,6 +44,7 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "kv_scale.h"
 #include "wl_ptx.cuh"
 
 namespace wl {
@@ -497,24 +498,11 @@ __global__ void __launch_bounds__(2 * RT * HB, 1024 / (2 * RT * HB)) kv_append_k
         const uint32_t m = s_top[part];
         const float nan = __uint_as_float(0x7FC00000u);
         const float need = m >= 0x7F800000u ? nan : __fdiv_rn(__uint_as_float(m), 127.0f);
-        float s = need;
-        int k = 0;
-        if (first != 0u) {
-            if (!(need == need) || !(old == old)) {
-                s = nan;
-            } else if (need <= old) {
-                s = old;
-            } else if (old != 0.0f) {
-                s = old;
-                while (s < need) {  // at most 2^8 + 2^5 doublings between two floats
-                    s *= 2.0f;
-                    ++k;
-                }
-            }
-        }
-        *scale = s;
-        s_scale[part] = s;
-        s_grow[part] = k;
+        PageScale g = {need, 0};
+        if (first != 0u) g = grown_scale(old, need);
+        *scale = g.scale;
+        s_scale[part] = g.scale;
+        s_grow[part] = g.doublings;
     }
     bar_named(1u + part, RT);
     const float s = s_scale[part];
@@ -537,7 +525,7 @@ __global__ void __launch_bounds__(2 * RT * HB, 1024 / (2 * RT * HB)) kv_append_k
         for (int it = 0; it < ITS; ++it) {
             const uint32_t row = from + r0 + it * rstep;
             if (row < rows) {
-                const uint2 w = s > 0.0f ? quantise8(x[it], s, inv) : make_uint2(0u, 0u);
+                const uint2 w = fabsf(s) > 0.0f ? quantise8(x[it], s, inv) : make_uint2(0u, 0u);
                 int8_t *to = codes + (size_t)(first + row) * D;
                 *reinterpret_cast<uint32_t *>(to + ea) = w.x;
                 *reinterpret_cast<uint32_t *>(to + eb) = w.y;

@@ -1,0 +1,50 @@
+"""Calls of the attention operators that their documentation allows at its edges, against the definitions in 64 bits
+(tests/attn_ref.py)."""
+import numpy as np
+import pytest
+import torch
+
+from attn_ref import Cache, append, append_args, append_ref, i32, rope_table, starts, status
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def randn(g, *shape, dtype=F32):
+    return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+
+@pytest.mark.parametrize("page,dim,n,first", [(32, 64, 1, 5), (16, 128, 3, 15), (128, 64, 90, 20)])
+def test_append_to_pages_with_negative_scales(page, dim, n, first):
+    """A page that other code filled with a negative scale keeps its sign and grows by its size: what is appended
+    is the mirror image of the same page with all signs turned."""
+    g = gen(page)
+    kv, need = 3, -(-(first + n) // page)
+    c = Cache(need + 1, page, kv, dim)
+    c.k.random_(-127, 128, generator=g)
+    c.v.random_(-127, 128, generator=g)
+    c.ks.uniform_(0.0005, 0.05, generator=g)
+    c.vs.uniform_(0.0005, 0.05, generator=g)
+    for size in (0.0, 0.3, 40.0):  # nothing new, values that fit, values that do not
+        k, v = randn(g, n, kv * dim) * size, randn(g, n, kv * dim) * size
+        rope = rope_table(first + n, 0)
+        table = [list(range(need))]
+        want, _, _, _ = append_ref(c, None, k, v, [n], [first], table, rope, 0, 0)
+        turned = c.clone()
+        for codes, scale in ((turned.k, turned.ks), (turned.v, turned.vs)):
+            codes[0, 1:].neg_()  # heads 1 and 2 of the begun page
+            scale[0, 1:].neg_()
+        append(turned, append_args(None, k, v, starts([n]), i32([first]), i32(table), None, 0, 0, F32, heads=kv))
+        torch.cuda.synchronize()
+        assert status() == 0
+        for got, ref in zip((turned.k, turned.ks, turned.v, turned.vs), want):
+            ref = torch.from_numpy(ref).cuda()
+            ref[0, 1:].neg_()
+            assert torch.equal(got, ref)
