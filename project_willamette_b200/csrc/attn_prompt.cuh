@@ -489,6 +489,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 2)
                 }
             }
             uint32_t again = __ballot_sync(0xffffffffu, mine && !fine);
+            __syncwarp();  // the lanes of prompt_row store over what the row's own lane stored
             while (again) {
                 const uint32_t k = __ffs(again) - 1u;
                 again &= again - 1u;

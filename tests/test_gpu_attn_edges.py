@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from attn_ref import Cache, append, append_args, append_ref, i32, rope_table, starts, status
+from attn_ref import (Cache, append, append_args, append_ref, i32, prompt, prompt_ref, rope_table, starts, status,
+                      within)
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +49,26 @@ def test_append_to_pages_with_negative_scales(page, dim, n, first):
             ref = torch.from_numpy(ref).cuda()
             ref[0, 1:].neg_()
             assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("dim,dtype,out", [(64, F16, F16), (128, BF16, BF16), (128, F16, F32), (64, BF16, F32)])
+def test_prompt_rows_computed_again(dim, dtype, out):
+    """An infinity and a NaN in the last value row: all rows before it in its tile are computed a second time, by
+    other threads than those that stored them first. What stays is the second result, every time."""
+    g = gen(dim)
+    heads, kv, lengths = 6, 2, [128, 300, 77]
+    T = sum(lengths)
+    q = randn(g, T, heads * dim, dtype=dtype)
+    k, v = randn(g, T, kv * dim, dtype=dtype), randn(g, T, kv * dim, dtype=dtype)
+    ref, tol = prompt_ref(q, k, v, lengths, heads, kv, dim, 0.1)
+    ends = np.cumsum(lengths) - 1
+    v[ends, 3], v[ends, dim + 5] = float("inf"), float("nan")
+    sees = torch.zeros(T, dtype=torch.bool, device="cuda")
+    sees[ends.tolist()] = True
+    first = None
+    for _ in range(20):
+        got = prompt(q, k, v, starts(lengths), heads, kv, dim, 0.1, out_type=out)
+        within(got[~sees], ref[~sees], tol[~sees])
+        first = got if first is None else first
+        assert torch.equal(got[~sees], first[~sees])
+    assert status() == 0
