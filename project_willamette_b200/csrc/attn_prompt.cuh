@@ -418,10 +418,12 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 2)
             if (j == 0) {
                 m = top;
             } else if (__any_sync(0xffffffffu, top > m + 8.0f)) {
+                // each row by its own maximum: one that has not risen so far keeps what it has
+                // (a factor of 1), so that no row's roundings depend on its neighbours
                 // the product of step j - 1 is done when the scores of step j + 1 are there
                 if (!wait_all(&s_full[(j + 1u) & 1u], ((j + 1u) >> 1) & 1u)) return false;
                 tc_fence_after();
-                const float mn = fmaxf(m, top);
+                const float mn = top > m + 8.0f ? top : m;
                 const float f = mn == -INFINITY ? 1.0f : ex2_approx(m - mn);
                 l *= f;
                 m = mn;

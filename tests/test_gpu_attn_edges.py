@@ -72,3 +72,27 @@ def test_prompt_rows_computed_again(dim, dtype, out):
         first = got if first is None else first
         assert torch.equal(got[~sees], first[~sees])
     assert status() == 0
+
+
+@pytest.mark.parametrize("dim,dtype,scale", [(64, F16, 0.125), (128, BF16, 0.09), (128, F16, -0.2)])
+def test_prompt_row_depends_on_what_it_sees_alone(dim, dtype, scale):
+    """Bit for bit: a row's result stays when the other rows' queries, the keys and values that its mask leaves out
+    and the neighbouring sequences change."""
+    g = gen(7 * dim)
+    heads, kv, n = 4, 2, 600
+    q = randn(g, n, heads * dim, dtype=dtype)
+    k, v = randn(g, n, kv * dim, dtype=dtype), randn(g, n, kv * dim, dtype=dtype)
+    alone = prompt(q, k, v, starts([n]), heads, kv, dim, scale, out_type=F32)
+    # every other query much larger, so that the running maxima of those rows climb far and often
+    big = q.clone()
+    big[1::2] *= 40
+    got = prompt(big, k, v, starts([n]), heads, kv, dim, scale, out_type=F32)
+    assert torch.equal(got[0::2], alone[0::2])
+    # later keys and values other and larger; packed between two other sequences
+    for keep in (n - 1, 570, 513, 512, 330, 64, 1):
+        a, b = k.clone(), v.clone()
+        a[keep:], b[keep:] = randn(g, n - keep, kv * dim, dtype=dtype) * 30, randn(g, n - keep, kv * dim, dtype=dtype) * 30
+        x, y, z = (torch.cat([randn(g, 77, t.shape[1], dtype=dtype) * 20, t, randn(g, 200, t.shape[1], dtype=dtype) * 20])
+                   for t in (q, a, b))
+        got = prompt(x, y, z, starts([77, n, 200]), heads, kv, dim, scale, out_type=F32)
+        assert torch.equal(got[77:77 + keep], alone[:keep])
