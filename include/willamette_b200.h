@@ -111,6 +111,8 @@ int wl_device_status(uint32_t *flags);
  * waits, grid barriers) on the current device, in ns; default 2 s, accepted
  * range [1 us, 600 s].  A wait that runs out sets bit 0 (or bit 1 for a peer
  * wait) of the device status word and its kernel returns; nothing hangs.
+ * The attention operators, before a CTA ends early, let its copies and products
+ * in flight end for a second at least, whatever the limit.
  * Synchronises the device; call it outside stream capture.  No counterpart
  * in the reference (its CPU path has no device waits). */
 int wl_set_wait_limit_ns(uint64_t ns);

@@ -745,10 +745,10 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
         joining = true;
         turn = following;
     }
-    // after a wait that ran out: (bounded) the copies still in flight land before
-    // the CTA's shared memory goes
+    // after a wait that ran out: the copies still in flight land before the CTA's shared
+    // memory goes
     if (lane == 0)
-        for (; it < issued; ++it) (void)mbar_wait(&s_full[warp][it % ST], (it / ST) & 1u);
+        for (; it < issued; ++it) mbar_drain(&s_full[warp][it % ST], (it / ST) & 1u);
 }
 
 }  // namespace wl

@@ -327,17 +327,17 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 2)
                 if (it >= 2u)
                     load_tile(dst + L::TILE / 2u, &maps.v, h, (uint32_t)begin + (it - 2u) * 64u, 64u, &kv_full[s]);
             }
-            // (bounded) the last copies land before the CTA's shared memory goes
-            (void)mbar_wait(&q_full, 0);
-            for (uint32_t k = it > ST ? it - ST : 0; k < it; ++k)
-                (void)mbar_wait(&kv_full[k % ST], (k / ST) & 1u);
+            // the last copies land before the CTA's shared memory goes
+            mbar_drain(&q_full, 0);
+            for (uint32_t k = it > ST ? it - ST : 0; k < it; ++k) mbar_drain(&kv_full[k % ST], (k / ST) & 1u);
         }
     } else if (warp == MMA_WARP) {
         if (lane == 0) {
             const uint32_t base = smem_u32(smem);
             const uint32_t bf = pack16<T>(1.0f, 0.0f) == 0x3F80u;
             const uint32_t idesc_s = umma_idesc_f16(bf, 0u, 64u), idesc_o = umma_idesc_f16(bf, 1u, D);
-            uint32_t freed = 0;  // ring entries whose reading is committed
+            uint32_t freed = 0;           // ring entries whose reading is committed
+            uint32_t told[2] = {0u, 0u};  // commits to s_full
             auto entry = [&](uint32_t it) { return base + (1u + it % ST) * L::TILE; };
             auto loaded = [&](uint32_t it) { return wait(&kv_full[it % ST], (it / ST) & 1u); };
             auto scores = [&](uint32_t s) {  // S = Q K^T of step s, into the place of its parity
@@ -353,6 +353,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 2)
                 tc_fence_after();
                 scores(s);
                 umma_commit(&s_full[s]);
+                told[s] = 1u;
                 umma_commit(&kv_empty[freed++ % ST]);
             }
             if (ok && n == 1u) {  // entry 1 holds nothing
@@ -371,11 +372,13 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 2)
                                 idesc_o, j != 0u || i != 0u);
                 if (j + 2u < n) scores(j + 2u);
                 umma_commit(&s_full[j & 1u]);  // of step j + 2, and that the product of step j is done
+                ++(j & 1u ? told[1] : told[0]);
                 umma_commit(&kv_empty[freed++ % ST]);
             }
-            // (bounded) every committed product is done before tensor memory goes
-            for (uint32_t k = freed > ST ? freed - ST : 0; k < freed; ++k)
-                (void)mbar_wait(&kv_empty[k % ST], (k / ST) & 1u);
+            // every committed product is done, and has said so, before tensor and shared memory go
+            for (uint32_t k = freed > ST ? freed - ST : 0; k < freed; ++k) mbar_drain(&kv_empty[k % ST], (k / ST) & 1u);
+            for (uint32_t i = 0; i < 2u; ++i)
+                if (told[i]) mbar_drain(&s_full[i], (told[i] - 1u) & 1u);
         }
     } else {
         const uint32_t r = tid;  // row in the tile

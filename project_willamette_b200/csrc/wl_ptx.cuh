@@ -74,6 +74,19 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
     return true;
 }
 
+// Before a CTA gives its shared or tensor memory back: wait for work on it that is issued
+// already and ends by itself (copies, committed products).  The limit is for waits on
+// others and may be as short as a microsecond, which a copy in flight outlasts; this one
+// waits a second at least, so that what the next CTA owns is not written to.  It is
+// bounded all the same.
+constexpr uint64_t WL_DRAIN_LEAST_NS = 1000000000ull;
+__device__ __forceinline__ void mbar_drain(uint64_t *bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity)) return;
+    const uint64_t t0 = globaltimer_ns(), limit = max(wait_limit_ns(), WL_DRAIN_LEAST_NS);
+    while (!mbar_try_wait(bar, parity) && globaltimer_ns() - t0 <= limit) {
+    }
+}
+
 // 1-D bulk copy of `bytes` (multiple of 16) from global memory into this
 // CTA's shared memory; both addresses 16-byte aligned.  Completion is
 // counted as transaction bytes on `bar`.

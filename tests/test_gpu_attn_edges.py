@@ -4,8 +4,9 @@ import numpy as np
 import pytest
 import torch
 
-from attn_ref import (Cache, append, append_args, append_ref, i32, prompt, prompt_ref, rope_table, starts, status,
-                      within)
+from attn_ref import (Cache, append, append_args, append_ref, check, decode, decode_ref, i32, prompt, prompt_ref,
+                      rope_table, starts, status, within, workspace)
+from project_willamette_b200 import _abi
 
 pytestmark = pytest.mark.gpu
 
@@ -96,3 +97,44 @@ def test_prompt_row_depends_on_what_it_sees_alone(dim, dtype, scale):
                    for t in (q, a, b))
         got = prompt(x, y, z, starts([77, n, 200]), heads, kv, dim, scale, out_type=F32)
         assert torch.equal(got[77:77 + keep], alone[:keep])
+
+
+def test_waits_that_run_out_leave_later_calls_right():
+    """With the shortest limit that the library takes, calls in good order may give up in the middle, with copies
+    and products in flight. They say so, and calls after them, on the same SMs, are right."""
+    g = gen(41)
+    page, heads, kv, dim = 64, 8, 2, 128
+    lengths = [9000, 400, 3000, 12000]
+    total = sum(-(-n // page) for n in lengths)
+    order = torch.randperm(total, generator=g, device="cuda").tolist()
+    most = max(-(-n // page) for n in lengths)
+    table = i32([[order.pop() for _ in range(-(-n // page))] + [0] * (most + (-n // page)) for n in lengths])
+    c = Cache(total, page, kv, dim)
+    c.k.random_(-127, 128, generator=g)
+    c.v.random_(-127, 128, generator=g)
+    c.ks.uniform_(0.002, 0.03, generator=g)
+    c.vs.uniform_(0.002, 0.03, generator=g)
+    q = randn(g, len(lengths), heads * dim)
+    dref, n = decode_ref(c, q, lengths, table, heads, 0.1), i32(lengths)
+    rows = [900, 128, 1500]
+    x, k, v = (randn(g, sum(rows), m * dim, dtype=BF16) for m in (heads, kv, kv))
+    pref = prompt_ref(x, k, v, rows, heads, kv, dim, 0.1)
+    L, start = _abi.lib(), starts(rows)
+    torch.cuda.synchronize()
+    assert status() == 0
+    for _ in range(20):
+        check(L.wl_set_wait_limit_ns(1000))
+        try:
+            a = decode(c, q, n, table, heads, 0.1)
+            b = prompt(x, k, v, start, heads, kv, dim, 0.1)
+            torch.cuda.synchronize()
+        finally:
+            check(L.wl_set_wait_limit_ns(2_000_000_000))
+        flags = status()
+        assert flags in (0, 1)
+        if not flags:
+            within(a, *dref)
+            within(b, *pref)
+        within(decode(c, q, n, table, heads, 0.1, ws=workspace(len(lengths), heads, c)), *dref)
+        within(prompt(x, k, v, start, heads, kv, dim, 0.1), *pref)
+        assert status() == 0
