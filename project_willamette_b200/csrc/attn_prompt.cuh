@@ -249,6 +249,10 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 2)
                          smem_u32(&s_tmem)),
                      "r"(PROMPT_COLUMNS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        // by this warp alone: the next kernel's CTAs may come once this one's tensor memory is
+        // allocated.  Before that they could take the columns and wait for this grid's end,
+        // which waits for the columns.
+        pdl_launch_dependents();
     }
     if (tid == 0) {
         mbar_init(&q_full, 1);
@@ -267,7 +271,6 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 2)
         const CUtensorMap *map = lane == 0u ? &maps.q : lane == 1u ? &maps.k : &maps.v;
         asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
     }
-    pdl_launch_dependents();
     pdl_wait();
     if (warp == TMA_WARP) {
         const SeqExtent e = find_extent(p.seq_start, nullptr, p.n_seqs, PROMPT_ROWS, 1u, unit, lane);

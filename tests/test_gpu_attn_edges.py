@@ -138,3 +138,25 @@ def test_waits_that_run_out_leave_later_calls_right():
         within(decode(c, q, n, table, heads, 0.1, ws=workspace(len(lengths), heads, c)), *dref)
         within(prompt(x, k, v, start, heads, kv, dim, 0.1), *pref)
         assert status() == 0
+
+
+def test_prompts_in_a_chain():
+    """Calls of both head sizes queued one behind another, each of several rounds of CTAs, so that a call's CTAs
+    come while the one before still runs: the same bits as each call by itself."""
+    g = gen(42)
+    calls = []
+    for heads, kv, dim, rows, dtype in [(9, 3, 64, [700, 1, 300, 900, 64], F16), (8, 2, 128, [1000, 129, 2000], BF16),
+                                        (20, 5, 128, [1], F16), (16, 16, 64, [513, 511, 1024], BF16)]:
+        x, k, v = (randn(g, sum(rows), m * dim, dtype=dtype) for m in (heads, kv, kv))
+        a = (x, k, v, starts(rows), heads, kv, dim, 0.1)
+        out = prompt(*a)
+        torch.cuda.synchronize()
+        within(out, *prompt_ref(x, k, v, rows, heads, kv, dim, 0.1))
+        calls.append((a, out, torch.empty_like(out)))
+    for _ in range(30):
+        for a, _, other in calls:
+            prompt(*a, out=other)
+    torch.cuda.synchronize()
+    assert status() == 0
+    for _, out, other in calls:
+        assert torch.equal(out, other)
