@@ -160,3 +160,80 @@ def test_prompts_in_a_chain():
     assert status() == 0
     for _, out, other in calls:
         assert torch.equal(out, other)
+
+
+@pytest.mark.parametrize("seqs,longest,heads,kv,dim,n_rot,pairs,dtype,out", [
+    (500, 12, 6, 2, 64, 64, 1, F32, F16), (500, 12, 6, 2, 64, 6, 0, F32, F32), (700, 9, 20, 5, 128, 120, 0, BF16, BF16),
+    (40, 300, 5, 5, 128, 10, 1, F16, F32), (1300, 140, 1, 1, 64, 64, 0, BF16, F16),
+])
+def test_append_queries_of_many_tokens(seqs, longest, heads, kv, dim, n_rot, pairs, dtype, out):
+    """More tokens than the GPU takes query CTAs at a time, so that one CTA rotates the queries of several: across
+    short and empty sequences, past one whose position is bad, with a shorter last CTA; the last case past the
+    largest number of tokens a CTA."""
+    g, page, P = gen(seqs), 32, np.random.default_rng(seqs)
+    lengths = P.integers(0, longest + 1, seqs)
+    lengths[P.integers(0, seqs, seqs // 4)] = 0
+    bad = seqs // 2
+    lengths[bad] = 5
+    position = P.integers(0, 2 * page, seqs)
+    position[bad] = 0
+    ctas = 6 * torch.cuda.get_device_properties(0).multi_processor_count
+    block = min(64, -(-int(lengths.sum()) // ctas))
+    lengths[-1] += lengths.sum() % block == 0
+    T = int(lengths.sum())
+    assert block > 1 and T % block and (seqs < 1300 or T > 64 * ctas)
+    need = [-(-(a + b) // page) for a, b in zip(lengths, position)]
+    order = P.permutation(sum(need)).tolist()
+    table = [[order.pop() for _ in range(m)] + [0] * (max(need) - m) for m in need]
+    c = Cache(sum(need), page, kv, dim, fill=9)
+    c.ks.uniform_(0.001, 0.05, generator=g)
+    c.vs.uniform_(0.001, 0.05, generator=g)
+    rope = rope_table(int(max(lengths + position)) + 1, n_rot)
+    q, k, v = (randn(g, T + 3, m * dim, dtype=dtype) for m in (heads, kv, kv))
+    want, rq, rk, rv = append_ref(c, q, k, v, lengths.tolist(), position.tolist(), table, rope, n_rot, pairs)
+    before = c.clone()
+    outs = [torch.full((T + 3, m * dim), 7.0, dtype=out, device="cuda") for m in (heads, kv, kv)]
+    given = position.copy()
+    given[bad] = -1
+    append(c, append_args(q, k, v, starts(lengths), i32(given.tolist()), i32(table), torch.from_numpy(rope).cuda(), n_rot,
+                          pairs, out, *outs, heads=heads))
+    torch.cuda.synchronize()
+    assert status() == 4
+    skip = table[bad][0]  # the page that the bad sequence would have written
+    for got, ref, old in zip((c.k, c.ks, c.v, c.vs), want, (before.k, before.ks, before.v, before.vs)):
+        ref = torch.from_numpy(ref).cuda()
+        ref[skip] = old[skip]
+        assert torch.equal(got, ref)
+    first = int(lengths[:bad].sum())
+    for got, ref in zip(outs, (rq, rk, rv)):
+        ref = torch.cat([torch.from_numpy(ref.reshape(T, -1)).to(out).cuda(), torch.full_like(got[T:], 7)])
+        ref[first:first + 5] = 7
+        assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("lengths,heads,kv,dim,dtype", [
+    ([3001], 8, 1, 64, F16), ([200, 4500], 12, 1, 128, BF16), ([8192], 2, 1, 128, F16), ([6001], 2, 2, 64, BF16),
+    ([1100, 1, 2049], 32, 4, 128, BF16), ([1500], 17, 1, 128, F16),
+])
+def test_prompt_long_and_wide_groups(lengths, heads, kv, dim, dtype):
+    g = gen(sum(lengths))
+    T = sum(lengths)
+    q = randn(g, T, heads * dim, dtype=dtype)
+    k, v = randn(g, T, kv * dim, dtype=dtype), randn(g, T, kv * dim, dtype=dtype)
+    within(prompt(q, k, v, starts(lengths), heads, kv, dim, dim ** -0.5, out_type=F32),
+           *prompt_ref(q, k, v, lengths, heads, kv, dim, dim ** -0.5))
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, F16), (128, BF16)])
+def test_prompt_maxima_that_rise_late(dim, dtype):
+    """Long stretches of like scores, then a rise past what went before, some thousand keys in and again at the end."""
+    g = gen(dim + 1)
+    heads, kv, n = 2, 1, 4200
+    q = randn(g, n, heads * dim, dtype=dtype) * 0.1 + 1
+    k = randn(g, n, dim) * 0.1
+    for at, size in ((1000, 0.1), (2500, 0.4), (2563, 0.8), (4133, 1.5)):
+        k[at:] += size
+    k, v = k.to(dtype), randn(g, n, dim, dtype=dtype)
+    for scale in (0.5, -0.5):
+        within(prompt(q, k, v, starts([n]), heads, kv, dim, scale, out_type=F32),
+               *prompt_ref(q, k, v, [n], heads, kv, dim, scale))
