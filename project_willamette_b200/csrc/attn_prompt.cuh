@@ -102,7 +102,9 @@ __device__ __forceinline__ void prompt_row(const AttnPromptParams &p, int64_t be
 // of step j is in the output.
 // The masked part of a product is 0 x v, which is NaN where v is not finite: a row whose
 // scores or output are not finite is computed again by prompt_row, which does not read
-// what the mask leaves out.
+// what the mask leaves out, unless one of its own scores is NaN, which makes all of it NaN.
+// That path is slow: where all rows take it (an infinity in an early value row of f16), 2048
+// tokens take 10 ms and 2 x 8192 take 99, 200 times as long.
 //
 // What bounds it: at D = 128 an SM's 128 keys of a tile take 1650 cycles of products (an
 // MMA of M = 128 takes 64 to 70 cycles for N = 64 as for N = 128) and 1030 of exponentials
@@ -389,6 +391,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 2)
         const float sc = p.scale * 1.4426950408889634f;
         float m = 0.0f, l = 0.0f;  // m: the maximum in use, in log2 units
         bool ok = true, fine = true;
+        bool none = false;  // a score that the row sees is NaN: so is its sum, and all of its output
         // one step; DIAG: of the last two, where row r sees keys 0 .. `seen` of the 64 (a code
         // path of its own, so that the others carry no masks)
         auto step = [&](uint32_t j, int seen, auto last) {
@@ -419,6 +422,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 2)
             }
             float top = sc >= 0.0f ? max3_nan(max3_nan(hi[0], hi[1], hi[2]), hi[3], hi[3])
                                    : min3_nan(min3_nan(lo[0], lo[1], lo[2]), lo[3], lo[3]);
+            none = none || top != top;
             top = DIAG && seen < 0 ? -INFINITY : top * sc;
             fine = fine && top < INFINITY;  // NaN or infinite scores: the row is computed again
             if (j == 0) {
@@ -496,7 +500,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 2)
                     if (mine) store8(p.out, p.out_type, at + i + k, x);
                 }
             }
-            uint32_t again = __ballot_sync(0xffffffffu, mine && !fine);
+            uint32_t again = __ballot_sync(0xffffffffu, mine && !fine && !none);
             __syncwarp();  // the lanes of prompt_row store over what the row's own lane stored
             while (again) {
                 const uint32_t k = __ffs(again) - 1u;

@@ -237,3 +237,32 @@ def test_prompt_maxima_that_rise_late(dim, dtype):
     for scale in (0.5, -0.5):
         within(prompt(q, k, v, starts([n]), heads, kv, dim, scale, out_type=F32),
                *prompt_ref(q, k, v, [n], heads, kv, dim, scale))
+
+
+@pytest.mark.parametrize("heads,kv,dim,dtype", [(20, 5, 128, F16), (9, 3, 64, BF16)])
+def test_prompt_of_nan_takes_no_longer(heads, kv, dim, dtype):
+    """A NaN key makes every row that sees it NaN, and a call with it takes the time of any other: such rows used to
+    be computed again one by one, which took over a hundred times as long."""
+    g = gen(43)
+    T, at = 2048, 3
+    q, k, v = (randn(g, T, m * dim, dtype=dtype) for m in (heads, kv, kv))
+    bad = k.clone()
+    bad[at] = float("nan")
+    start, out = starts([T]), torch.empty(T, heads * dim, dtype=dtype, device="cuda")
+    got = prompt(q, bad, v, start, heads, kv, dim, 0.1)
+    assert torch.isnan(got[at:]).all()
+    assert torch.equal(got[:at], prompt(q, k, v, start, heads, kv, dim, 0.1)[:at])
+
+    def shortest(keys):
+        times = []
+        for _ in range(5):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(4):
+                prompt(q, keys, v, start, heads, kv, dim, 0.1, out=out)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    assert shortest(bad) < 20 * shortest(k)
