@@ -211,6 +211,34 @@ def test_append_queries_of_many_tokens(seqs, longest, heads, kv, dim, n_rot, pai
         assert torch.equal(got, ref)
 
 
+def test_append_outputs_beside_bad_indexes():
+    """A page id out of range keeps that page out of the cache and nothing else: the tokens' rotated queries, keys
+    and values are written. A bad position keeps all rows of its sequence as they were."""
+    g, page, heads, kv, dim = gen(44), 16, 4, 2, 64
+    lengths, table = [20, 7, 18], [[0, 1], [2, 3], [4, 5]]
+    T, rope = sum(lengths), rope_table(64, dim)
+    q, k, v = (randn(g, T, m * dim) for m in (heads, kv, kv))
+    for bad_page, bad_position in ((True, False), (False, True)):
+        c = Cache(6, page, kv, dim, fill=55)
+        want, rq, rk, rv = append_ref(c, q, k, v, lengths, [0, 0, 0], table, rope, dim, 0)
+        outs = [torch.full((T, m * dim), 7.0, device="cuda") for m in (heads, kv, kv)]
+        given = [[0, 1], [2, 3], [4, 6 if bad_page else 5]]
+        append(c, append_args(q, k, v, starts(lengths), i32([0, 64 if bad_position else 0, 0]), i32(given),
+                              torch.from_numpy(rope).cuda(), dim, 0, F32, *outs, heads=heads))
+        torch.cuda.synchronize()
+        assert status() == 4
+        out = 5 if bad_page else 2  # the page that stays as it was
+        assert (c.k[out] == 55).all() and (c.v[out] == 55).all() and (c.ks[out] == 0).all()
+        for got, ref in zip((c.k, c.ks, c.v, c.vs), want):
+            for p in set(range(6)) - {out}:
+                assert torch.equal(got[p].cpu(), torch.from_numpy(ref[p]))
+        for got, ref in zip(outs, (rq, rk, rv)):
+            ref = torch.from_numpy(ref.reshape(T, -1)).cuda()
+            if bad_position:
+                ref[20:27] = 7
+            assert torch.equal(got, ref)
+
+
 @pytest.mark.parametrize("lengths,heads,kv,dim,dtype", [
     ([3001], 8, 1, 64, F16), ([200, 4500], 12, 1, 128, BF16), ([8192], 2, 1, 128, F16), ([6001], 2, 2, 64, BF16),
     ([1100, 1, 2049], 32, 4, 128, BF16), ([1500], 17, 1, 128, F16),
