@@ -102,10 +102,13 @@ int wl_init(int device);
 int wl_release_weights(void);
 /* Device-side error word (bit 0: a bounded wait timed out; bit 1: a
  * tensor-parallel peer never arrived; bit 2: an attention operator read a
- * page id, position, length or sequence extent outside its range).  Synchronises the device, then reads
- * and clears it.  Includes the status word of wl_dev_i2s_matvec_f32_noalloc
- * on the calling thread's current device; when only that entry point has run
- * in the process, this call allocates nothing either. */
+ * page id, position, length or sequence extent outside its range).
+ * Synchronises the device, then reads and clears it.  Includes the status word
+ * of wl_dev_i2s_matvec_f32_noalloc on the calling thread's current device; when
+ * only that entry point has run in the process, this call allocates nothing
+ * either.  A BitNet engine's call uses bits 2 to 4 for itself (non-finite
+ * hidden state, cache full, grid stopped) and takes them back before it
+ * returns: they are seen here only by a thread that asks meanwhile. */
 int wl_device_status(uint32_t *flags);
 /* Limit of every bounded device-side wait (TMA stage waits, peer and flag
  * waits, grid barriers) on the current device, in ns; default 2 s, accepted
@@ -349,8 +352,9 @@ int wl_dev_i2s_matvec_f32_noalloc(const uint8_t *packed, float w_scale, uint32_t
  * (q, k, v, out) hold token t's heads side by side at t * stride elements;
  * they are 16-byte aligned, strides multiples of 16 bytes, so that slices of
  * one fused projection work.  Page ids, positions, lengths and seq_start are
- * read on the device: a value outside its range is left out and sets bit 2
- * of wl_device_status, never followed. */
+ * read on the device: a value outside its range is never followed and sets bit
+ * 2 of wl_device_status.  What becomes of the rows that it stands for is said
+ * at each call. */
 
 /* A paged int8 cache: page p, KV head h holds rows [page_size][head_dim] of
  * codes at ((p * n_kv_heads + h) * page_size) * head_dim, in K and in V, and one
@@ -389,7 +393,10 @@ typedef struct wl_kv_pages_i8 {
  * rounded once to out_type; they must not overlap q, k or v.  q and q_out may
  * both be NULL.
  * A page may be written for one sequence only in a call, and calls on one
- * cache must not overlap on the GPU. */
+ * cache must not overlap on the GPU.
+ * A sequence whose extent or position is out of range is left out: its pages
+ * and its rows of q_out, k_out and v_out stay as they were.  For a page id out
+ * of range only that page is: the tokens' q_out, k_out and v_out are written. */
 typedef struct wl_kv_append {
     const void *q, *k, *v;     /* device, type `type` */
     uint64_t q_stride, k_stride, v_stride; /* elements between tokens */
@@ -407,7 +414,12 @@ int wl_dev_rope_kv_append_i8(const wl_kv_pages_i8 *cache, const wl_kv_append *ar
 
 /* Attention of one token per sequence over its first length[s] positions of
  * the cache: out = softmax(scale * q . k) v for each query head, zeros where
- * length[s] is 0.  Softmax and sums in f32.  workspace:
+ * length[s] is 0 or out of range; the keys of a page id out of range take no
+ * part.  Softmax and sums in f32.  The weights enter the product with v
+ * with 22 bits, relative to the largest weight and the largest scale among the
+ * sequence's pages of v: a weight below 2^-39 of both together is lost, so pages
+ * whose scales differ by more than 2^15 or so cost digits.  out must not overlap
+ * q.  workspace:
  * wl_attn_decode_workspace_bytes bytes, 16-byte aligned, zero before the first
  * call; every call leaves its counters zero again (zero it anew after a call
  * whose wait timed out, bit 0 of wl_device_status).  Calls that share a
@@ -432,11 +444,17 @@ int wl_dev_attn_decode_i8(const wl_kv_pages_i8 *cache, const wl_attn_decode *arg
 /* Causal attention within packed prompts: row i of sequence s (rows
  * seq_start[s] .. seq_start[s + 1] of q, k, v) attends to rows 0 .. i of the
  * same sequence.  Sequences are begun in the caller's order: long prompts are
- * best put first.  What masked rows hold, NaN included, has no effect.  Rows
- * of out that no sequence owns are left as they were.  q, k and v are all
+ * best put first.  What masked rows hold, NaN included, has no effect, and a
+ * row's bits do not depend on the sequences beside it.  (Next to masked NaN or
+ * infinities a row is computed another way, within the same error.)  Rows
+ * of out that no sequence owns, and those of a sequence whose extent is out of
+ * range, are left as they were.  q, k and v are all
  * WL_GGML_F16 or all WL_GGML_BF16; out is that type or WL_GGML_F32.  Scores,
  * softmax and sums in f32; the weights enter the product with v in the
- * inputs' 16-bit type.  out must not overlap q, k or v. */
+ * inputs' 16-bit type.  out must not overlap q, k or v.  A row that is not
+ * finite, and not for a NaN score, is computed again on a slow path: where an
+ * infinity in an early row of v reaches most rows, the call takes about 200
+ * times as long. */
 typedef struct wl_attn_prompt {
     const void *q, *k, *v;     /* device */
     void *out;                 /* device */

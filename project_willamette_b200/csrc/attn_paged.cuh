@@ -25,13 +25,16 @@
 // ring of its own, across its segments.  An item cut between CTAs is joined by the last
 // CTA to arrive, in CTA order, so results repeat.
 //
-// Bound by HBM: 2 bytes a key, head and dimension, 4 G flops each; in the steady state the
-// copies run near a plain copy's rate (6.55 TB/s), and what is left is a call's beginning
-// and end (about 9 us, all of a small call).  Measured (median call in a captured chain):
-// 64 sequences to 8192 keys, 5 KV heads of 128, 65.9 us = 4.41 TB/s (0.67 of the copy); 4
-// sequences to 100,000 keys, 4 KV heads, 74.2 us = 4.67 TB/s; 32 sequences to 1024 keys, 3
-// KV heads of 64, 9.8 us; one of 640 keys, 5 heads of 128, 9.0 us.  Three CTAs an SM at
-// 168 registers (spilling) instead of two at 212: 64.8, 75.2, 10.1 and 10.7; rings of 24
+// Bound by HBM: 2 bytes a key, head and dimension, 4 G flops each.  Over growing lengths the
+// time rises at 5.8 TB/s (64 equal sequences of 1024 to 16384 keys, 5 KV heads of 128: 28.0,
+// 43.0, 71.3, 128.5, 246.4 us; 4 of 12,500 to 200,000, 4 KV heads: 24.1 to 155.6), 0.88 of a
+// plain copy's 6.55: no pipe is full, a warp's chain for one tile and the borders between
+// segments hold it.  The rest is a call's beginning and end, 13 to 15 us of such calls and
+// 9 of a small one.  Measured (median call in a captured chain; in ordinary launches back to
+// back in brackets): 64 sequences to 8192 keys, 5 KV heads of 128, 65.8 us (68.4) = 4.42
+// TB/s; 4 sequences to 100,000 keys, 4 KV heads, 74.3 us (79.0) = 4.67 TB/s; 32 sequences to
+// 1024 keys, 3 KV heads of 64, 9.8 us; one of 640 keys, 5 heads of 128, 9.0 us.  Three CTAs an
+// SM at 168 registers (spilling) instead of two at 212: 64.8, 75.2, 10.1 and 10.7; rings of 24
 // KB a warp instead of 16 at D = 128: 67.6, 76.9; rings of 16 KB instead of 24 at D = 64:
 // 10.3 for 9.8; CTAs without a place not launched: 9.25 to 9.0.  Steps on the way at 64 x
 // 8192: one CTA a (query head, sequence) on the CUDA cores 6169 us; tiles from registers
@@ -471,7 +474,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, PAGED_CTAS_PER_SM)
         if (more) {
             // the pass's query rows: row g as f16 parts hi (tile row g) and lo (row
             // g + 8) of q * 2^shift, its largest |q| brought to [2^13, 2^14).  Kept in
-            // shared memory: in registers they measured the same (66.5 us for 65.9)
+            // shared memory: in registers they measured 9.2, 9.7, 66.5 and 74.6 us against
+            // 9.0, 9.8, 65.9 and 74.2 (one of 640 keys, 32 to 1024, 64 to 8192, 4 to 100,000)
             const PagedSegment &sg = s_sg[turn];
             if (joining) begin_segment(sg);
             uint4 raw[D / 16];

@@ -109,12 +109,13 @@ __device__ __forceinline__ void prompt_row(const AttnPromptParams &p, int64_t be
 // What bounds it: at D = 128 an SM's 128 keys of a tile take 1650 cycles of products (an
 // MMA of M = 128 takes 64 to 70 cycles for N = 64 as for N = 128) and 1030 of exponentials
 // (16 a cycle and SM), a softmax warp 2400 from scores to weights, and two CTAs overlap
-// these to about 1750; long prompts also run into the power limit (2 x 8192: 544 to 600 us
-// by the run).  At D = 64 the softmax alone bounds it.  Short prompts pay each CTA's
-// beginning and end, 6000 cycles.  Measured (median call in a captured chain): 2 prompts to
-// 8192 tokens, 20 / 5 heads of 128, bf16, 544 us = 1106 TFLOP/s of the causal half (0.66
-// of cuBLAS's dense rate); 2048 tokens f16 35.8 us; 32 packed prompts to 1024 tokens, 9 / 3
-// heads of 64, 49.4 us; 77 tokens 6.0 us.
+// these to about 1750; long prompts also run into the power limit.  At D = 64 the softmax
+// alone bounds it.  Short prompts pay each CTA's beginning and end, 6000 cycles.  Measured
+// (median call in a captured chain; in ordinary launches back to back in brackets): 2
+// prompts to 8192 tokens, 20 / 5 heads of 128, bf16, 541 to 592 us by the run (638, at 1560 MHz
+// under the power limit: 944 TFLOP/s of the causal half, 0.68 of cuBLAS's sustained dense
+// rate); 2048 tokens f16 36.0 us (37.8); 32 packed prompts to 1024 tokens, 9 / 3 heads of 64,
+// 49.5 us (49.8); 77 tokens 6.0 us (7.4, the host's launches).
 // Steps on the way, at 2 x 8192: rows on the CUDA cores 100.8 ms; two tiles a CTA of 10
 // warps, 128-key steps 654 us; the masked last step a code path of its own (its 128
 // predicates had been kept in registers through every step) 581; one tile a CTA, two CTAs

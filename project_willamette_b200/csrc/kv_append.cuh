@@ -32,10 +32,13 @@
 // Measured (median call in a captured chain): 64 single tokens, 20 / 5 heads of 128 in f32,
 // 4.4 us, of 32 with 9 / 3 heads of 64 3.7 us (a launch and its dependent loads); 512
 // tokens with f16 copies 10.7 us; 14,845 bf16 tokens, 32 / 8 heads of 128, pages of 16,
-// with copies, 98 us = 4.02 TB/s (0.61 of a plain copy; 64 % of the issue slots, mostly
-// conversions and addresses).  Queries in the page CTAs and one head a CTA took 141 us; a
-// query warp's pieces share one table piece, and 64 registers (four CTAs of 256) beat
-// 80 or 120 with more loads in flight (98 against 109 and 217).
+// with copies, 98 us = 4.02 TB/s of inputs and outputs (0.61 of a plain copy; through DRAM
+// 3.5, the last outputs stay in L2).  64 % of the issue slots are taken: conversions,
+// addresses, and the spills of this instance (104 bytes stored and 156 loaded a thread).
+// Queries in the page CTAs and one head a CTA took 141 us; a query warp's pieces share one
+// table piece, and 64 registers (four CTAs of 256) beat 80 or 120 with more loads in flight
+// (98 against 109 and 217).  At 512 tokens 40 page CTAs with work stand behind 512 of
+// queries that hold one token each.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -388,7 +391,7 @@ __device__ __forceinline__ uint2 quantise8(const float (&x)[8], float s, float i
     for (int i = 0; i < 8; ++i) {
         v[i] = x[i] * inv;
         const float d = fabsf(v[i] - ((v[i] + MAGIC) - MAGIC));
-        far = d <= far ? far : d;  // NaN stays
+        far = d <= far ? far : d;  // an infinite `inv` makes all eight NaN, the last one too
     }
     if (!(far < 0.4999f)) {
 #pragma unroll
